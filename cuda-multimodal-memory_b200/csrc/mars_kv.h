@@ -1,0 +1,40 @@
+// mars_kv.h -- host-side context of the paged key/value cache operators
+// (mars_kv.cu: lengths to tables, mars_rope.cu: rotary positions and cache
+// writes, mars_attn*.cu: attention over the pages).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "mars_b200.h"
+#include "mars_internal.h"
+
+struct mars_kv_ctx {
+    int32_t device = 0;
+    int32_t max_requests = 0;
+    int32_t num_sms = 0;
+    cudaStream_t stream = nullptr;
+
+    // Arrival counters (kTicket*), zero between calls: a call's last block
+    // puts back the one it used.
+    unsigned int* d_tickets = nullptr;
+
+    // The working memory above holds one call at a time.  `used` is recorded
+    // after every call outside a capture; a call on another stream waits for it.
+    cudaStream_t last = nullptr;
+    cudaEvent_t used = nullptr;
+    bool any = false;
+};
+
+namespace mars {
+
+constexpr int kTicketRelease = 0;
+constexpr int kTicketPlan = 1;
+constexpr int kKvTickets = 2;
+
+// The stream of a call on `c`, ordered after the context's previous call.
+int kv_begin(mars_kv_ctx* c, void* stream, cudaStream_t* st);
+// Marks the end of the call's work on `st`.
+int kv_end(mars_kv_ctx* c, cudaStream_t st);
+
+}  // namespace mars

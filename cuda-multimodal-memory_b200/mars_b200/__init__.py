@@ -166,6 +166,13 @@ _SIGS = {
     "mars_scan_topk_noalloc": [_VP, _I32, _VP, _VP, _VP, _I32, _I32, _VP, _F32, _F32, _I32, _I32,
                                _I32, _I32, _VP, _VP, _VP, _VP],
 }
+_SIGS.update({
+    "mars_kv_ctx_create": [_I32, _I32, C.POINTER(_VP)],
+    "mars_kv_ctx_destroy": [_VP],
+    "mars_kv_release": [_VP, _I32, _VP, _VP, _VP, _I32, _I32, _VP, _I32, _VP, _VP, _VP, _VP, _VP],
+    "mars_kv_plan": [_VP, _I32, _VP, _VP, _VP, _I32, _I32, _VP, _I32, _VP, _I32, _VP, _VP, _VP, _VP, _VP, _VP,
+                     _VP],
+})
 _RESTYPE = {"mars_last_error": C.c_char_p, "mars_status_string": C.c_char_p,
             "mars_abi_version": C.c_int, "mars_query_ctx_stream": C.c_void_p}
 
@@ -709,3 +716,16 @@ def query_once(store: Store, q, t_q, cfg: RetrievalConfig | None = None):
     _check(lib().mars_query_once(store.handle, _ptr(qa), float(t_q), C.byref(cfg),
                                  out.ctypes.data, C.byref(n), None))
     return out[:n.value]
+
+
+# the operators of the answering step (kv.py) work on torch tensors and import
+# torch, so their module is loaded with the first of these names
+_KV_NAMES = ("KvContext", "KvPlan", "KV_MAX_REQUESTS", "KV_BAD_LENGTH", "KV_NO_PAGES", "KV_TABLE_FULL",
+             "KV_TOO_MANY_TOKENS", "KV_STACK_FULL")
+
+
+def __getattr__(name):
+    if name in _KV_NAMES:
+        from . import kv
+        return getattr(kv, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

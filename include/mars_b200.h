@@ -585,6 +585,63 @@ int mars_scan_topk_noalloc(const float* d_embeddings, int32_t row_pitch,
                            int32_t row_offset, int32_t* d_ids, float* d_vals,
                            int32_t* d_count, void* stream);
 
+/* ---- answering with memories: a paged key/value cache -------------------
+ * No reference counterpart: the reference retrieves memories and leaves the
+ * answer to its caller.  These are the operators of that caller's attention
+ * layers: it keeps the keys and values of its requests (retrieved memories
+ * first, then the conversation) in pages of page_size tokens, and every step
+ * adds new tokens to some requests -- one token each while it generates, a
+ * chunk or a whole prompt before.  A step is mars_kv_release (optional) and
+ * mars_kv_plan once, then mars_rope_append and mars_paged_attention in every
+ * layer.  All pointers are device pointers, all calls asynchronous on
+ * `stream` (NULL: the context's stream).  A context holds the working memory
+ * of one call at a time: calls on several streams are ordered one after the
+ * other (inside a stream capture, by the order of the launches of the graph). */
+#define MARS_KV_MAX_REQUESTS 8192
+typedef struct mars_kv_ctx mars_kv_ctx;
+
+/* Working memory for calls of up to max_requests requests. */
+int mars_kv_ctx_create(int32_t device, int32_t max_requests, mars_kv_ctx** out);
+/* Waits for the context's last call.  NULL is accepted. */
+int mars_kv_ctx_destroy(mars_kv_ctx* ctx);
+
+/* Bits of *d_status of mars_kv_release and mars_kv_plan (0: done).  A call
+ * that sets one leaves tables, stack, lengths and counts as they were, and
+ * hands out no token (d_cu_new all 0, d_slots and d_positions all -1). */
+enum {
+    MARS_KV_BAD_LENGTH      = 1,   /* a negative length, or one beyond 2^31 - 1 */
+    MARS_KV_NO_PAGES        = 2,   /* fewer free pages than the new tokens need */
+    MARS_KV_TABLE_FULL      = 4,   /* a request outgrows its table's row        */
+    MARS_KV_TOO_MANY_TOKENS = 8,   /* more new tokens than max_tokens           */
+    MARS_KV_STACK_FULL      = 16,  /* the free stack's count is outside [0, free_cap] */
+};
+
+/* Gives back the pages of the requests b with d_release[b] != 0: pushes
+ * d_tables[b][0 .. ceil(len / page_size)) onto the stack of free pages
+ * (d_free_pages[0 .. *d_free_count), room for free_cap) in the order of the
+ * requests, and sets their length to 0.  d_kv_lens_out / d_free_count_out
+ * may be the input arrays; the tables stay as they are.  d_status may be
+ * NULL. */
+int mars_kv_release(mars_kv_ctx* ctx, int32_t B, const int32_t* d_kv_lens, const int32_t* d_release,
+                    const int32_t* d_tables, int32_t table_pitch, int32_t page_size,
+                    int32_t* d_free_pages, int32_t free_cap, const int32_t* d_free_count,
+                    int32_t* d_kv_lens_out, int32_t* d_free_count_out, int32_t* d_status, void* stream);
+
+/* Room for d_new_lens[b] more tokens of request b, whose cache holds
+ * d_kv_lens[b]: pages are taken off the end of the free stack, request by
+ * request, into the next columns of d_tables (B rows of table_pitch).
+ * Outputs: d_kv_lens_out[b] = old + new; d_free_count_out; d_cu_new[B + 1],
+ * the new tokens before each request; and for token i of the call its slot
+ * d_slots[i] = page * page_size + offset and d_positions[i] (may be NULL),
+ * its place in its request.  d_slots and d_positions have max_tokens entries,
+ * -1 past the last token.  Output lengths and count may be the input arrays.
+ * Slots are 32-bit: the cache holds at most 2^31 - 1 tokens. */
+int mars_kv_plan(mars_kv_ctx* ctx, int32_t B, const int32_t* d_kv_lens, const int32_t* d_new_lens,
+                 int32_t* d_tables, int32_t table_pitch, int32_t page_size, const int32_t* d_free_pages,
+                 int32_t free_cap, const int32_t* d_free_count, int32_t max_tokens,
+                 int32_t* d_kv_lens_out, int32_t* d_free_count_out, int32_t* d_cu_new, int32_t* d_slots,
+                 int32_t* d_positions, int32_t* d_status, void* stream);
+
 /* Diagnostic: the fused score of every row (same arithmetic as the scan),
  * d_out: N floats, -FLT_MAX for rows rejected by the filter. */
 int mars_debug_fused_scores(const mars_store* s, mars_query_ctx* ctx,
