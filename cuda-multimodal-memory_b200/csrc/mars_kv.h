@@ -36,5 +36,7 @@ constexpr int kKvTickets = 2;
 int kv_begin(mars_kv_ctx* c, void* stream, cudaStream_t* st);
 // Marks the end of the call's work on `st`.
 int kv_end(mars_kv_ctx* c, cudaStream_t st);
+// Sizes and type of a cache that a call names.
+int check_cache(const mars_kv_cache* c, const char* fn);
 
 }  // namespace mars

@@ -97,6 +97,7 @@ class CmngConfig(C.Structure):
 _VP = C.c_void_p
 _I32 = C.c_int32
 _F32 = C.c_float
+_I64 = C.c_int64
 
 # name -> argtypes (all return int status unless listed in _RESTYPE)
 _SIGS = {
@@ -172,6 +173,9 @@ _SIGS.update({
     "mars_kv_release": [_VP, _I32, _VP, _VP, _VP, _I32, _I32, _VP, _I32, _VP, _VP, _VP, _VP, _VP],
     "mars_kv_plan": [_VP, _I32, _VP, _VP, _VP, _I32, _I32, _VP, _I32, _VP, _I32, _VP, _VP, _VP, _VP, _VP, _VP,
                      _VP],
+    "mars_rope": [_VP, _I32, _VP, _I64, _I64, _VP, _I64, _I64, _I32, _I32, _I32, _VP, _I32, _VP],
+    "mars_rope_append": [_VP, _VP, _VP, _I64, _I64, _VP, _I64, _I64, _VP, _I64, _I64, _VP, _I64, _I64, _I32, _I32,
+                         _VP, _VP, _VP],
 })
 _RESTYPE = {"mars_last_error": C.c_char_p, "mars_status_string": C.c_char_p,
             "mars_abi_version": C.c_int, "mars_query_ctx_stream": C.c_void_p}
@@ -720,7 +724,7 @@ def query_once(store: Store, q, t_q, cfg: RetrievalConfig | None = None):
 
 # the operators of the answering step (kv.py) work on torch tensors and import
 # torch, so their module is loaded with the first of these names
-_KV_NAMES = ("KvContext", "KvPlan", "KV_MAX_REQUESTS", "KV_BAD_LENGTH", "KV_NO_PAGES", "KV_TABLE_FULL",
+_KV_NAMES = ("KvCache", "KvContext", "KvPlan", "rope", "rope_append", "KV_MAX_REQUESTS", "KV_BAD_LENGTH", "KV_NO_PAGES", "KV_TABLE_FULL",
              "KV_TOO_MANY_TOKENS", "KV_STACK_FULL")
 
 

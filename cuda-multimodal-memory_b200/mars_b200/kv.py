@@ -4,6 +4,11 @@ A step of a program that answers with retrieved memories:
 
     lens, count = ctx.release(lens, finished, tables, free, count, page_size=64)
     plan = ctx.plan(lens, new_lens, tables, free, count, page_size=64, max_tokens=n)
+    for each layer, with q, k, v its new tokens' projections:
+        q = rope_append(q, k, v, positions, freq, axis, cache, plan.slots)
+
+rope is the rotation by itself, for programs that train; its gradient is
+rope(..., inverse=True) of the output's gradient.
 
 All arguments are torch CUDA tensors; calls run on torch's current stream
 unless one is given, and return without waiting.
@@ -44,6 +49,103 @@ def _ints(name, t, n=None, dims=1):
     if n is not None and t.shape[0] != n:
         raise ValueError(f"{name} must have {n} entries, has {t.shape[0]}")
     return t.data_ptr()
+
+
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # MARS_DTYPE_*
+
+
+class _Cache(C.Structure):
+    """mars_kv_cache."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int32), ("num_pages", C.c_int32),
+                ("page_size", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("reserved", C.c_int32),
+                ("k_strides", C.c_int64 * 3), ("v_strides", C.c_int64 * 3)]
+
+
+class _Table(C.Structure):
+    """mars_rope_table."""
+    _fields_ = [("freq", C.c_void_p), ("axis", C.c_void_p), ("rot_dim", C.c_int32), ("n_axes", C.c_int32),
+                ("interleaved", C.c_int32), ("reserved", C.c_int32)]
+
+
+class KvCache:
+    """The caller's pages: k and v are [pages, page_size, kv_heads, head_dim] CUDA tensors (fp16 or bf16) of any
+    strides with contiguous columns -- a permuted view where memory has the heads before the tokens."""
+
+    def __init__(self, k, v):
+        if k.shape != v.shape or k.dtype is not v.dtype or k.dim() != 4 or k.device != v.device or not k.is_cuda:
+            raise ValueError("k and v must be CUDA tensors [pages, page_size, kv_heads, head_dim] of one shape and type")
+        if k.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError("the cache holds fp16 or bf16")
+        ks, vs = k.stride(), v.stride()
+        if ks[3] != 1 or vs[3] != 1:
+            raise ValueError("the cache's columns must be contiguous")
+        self.k, self.v = k, v
+        pages, page, heads, dim = k.shape
+        self._c = _Cache(k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype], pages, page, heads, dim, 0,
+                         (C.c_int64 * 3)(*ks[:3]), (C.c_int64 * 3)(*vs[:3]))
+
+
+def _heads(name, x, like=None):
+    """Checks [tokens, heads, head_dim] with contiguous columns; the (token, head) strides."""
+    if x.dim() != 3 or not x.is_cuda or (x.stride(2) != 1 and x.shape[2] != 1):
+        raise ValueError(f"{name} must be a CUDA tensor [tokens, heads, head_dim] with contiguous columns")
+    if like is not None and (x.shape[0] != like.shape[0] or x.dtype is not like.dtype or x.device != like.device):
+        raise ValueError(f"{name} must have {like.shape[0]} tokens of {like.dtype}")
+    return x.stride(0), x.stride(1)
+
+
+def _table(tokens, positions, freq, axis, interleaved):
+    _ints("positions", positions, tokens, positions.dim())
+    if positions.dim() not in (1, 2):
+        raise ValueError("positions must be [tokens] or [tokens, axes]")
+    if freq.dtype is not torch.float32 or not freq.is_cuda or not freq.is_contiguous() or freq.dim() != 1:
+        raise ValueError("freq must be a contiguous float32 CUDA tensor of 1 dimension")
+    _ints("axis", axis, freq.shape[0])
+    axes = 1 if positions.dim() == 1 else positions.shape[1]
+    return _Table(freq.data_ptr(), axis.data_ptr(), 2 * freq.shape[0], axes, int(interleaved), 0)
+
+
+def rope(x, positions, freq, axis, *, interleaved=False, inverse=False, out=None, stream=None):
+    """Rotary positions of x [tokens, heads, head_dim] (fp32, fp16 or bf16): pair i turns by positions[:, axis[i]]
+    * freq[i].  positions: int32 [tokens, axes].  inverse: turns back, the gradient of the forward rotation."""
+    xt, xh = _heads("x", x)
+    if x.dtype not in _DTYPES:
+        raise ValueError("x must be fp32, fp16 or bf16")
+    table = _table(x.shape[0], positions, freq, axis, interleaved)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    yt, yh = _heads("out", out, x)
+    if out.shape != x.shape:
+        raise ValueError("out must have x's shape")
+    with torch.cuda.device(x.device):
+        _check(lib().mars_rope(C.byref(table), _DTYPES[x.dtype], x.data_ptr(), xt, xh, out.data_ptr(), yt, yh,
+                               x.shape[0], x.shape[1], x.shape[2], positions.data_ptr(), int(inverse),
+                               _stream(stream, x)))
+    return out
+
+
+def rope_append(q, k, v, positions, freq, axis, cache, slots, *, interleaved=False, out=None, stream=None):
+    """q rotated (returned, or into out, which may be q), k rotated and v copied into the cache's slots.
+    q: [tokens, q_heads, head_dim], k and v: [tokens, kv_heads, head_dim], all of the cache's type."""
+    qt, qh = _heads("q", q)
+    kt, kh = _heads("k", k, q)
+    vt, vh = _heads("v", v, q)
+    if q.dtype is not cache.k.dtype or k.shape[1:] != cache.k.shape[2:] or v.shape != k.shape or \
+            q.shape[2] != k.shape[2] or q.device != cache.k.device:
+        raise ValueError("q, k and v must have the cache's type, device, heads and columns")
+    table = _table(q.shape[0], positions, freq, axis, interleaved)
+    _ints("slots", slots, q.shape[0])
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ot, oh = _heads("out", out, q)
+    if out.shape != q.shape:
+        raise ValueError("out must have q's shape")
+    with torch.cuda.device(q.device):
+        _check(lib().mars_rope_append(
+            C.byref(table), C.byref(cache._c), q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
+            out.data_ptr(), ot, oh, q.shape[0], q.shape[1], positions.data_ptr(), slots.data_ptr(),
+            _stream(stream, q)))
+    return out
 
 
 class KvContext:

@@ -642,6 +642,61 @@ int mars_kv_plan(mars_kv_ctx* ctx, int32_t B, const int32_t* d_kv_lens, const in
                  int32_t* d_kv_lens_out, int32_t* d_free_count_out, int32_t* d_cu_new, int32_t* d_slots,
                  int32_t* d_positions, int32_t* d_status, void* stream);
 
+/* The cache in the caller's memory: token `offset` of page p, head h starts
+ * at k + p * k_page_stride + offset * k_slot_stride + h * k_head_stride (all
+ * strides in elements, the head_dim elements contiguous; v likewise).  Slot s
+ * of mars_kv_plan is token s % page_size of page s / page_size. */
+enum { MARS_DTYPE_F32 = 0, MARS_DTYPE_F16 = 1, MARS_DTYPE_BF16 = 2 };
+typedef struct mars_kv_cache {
+    void*   k;
+    void*   v;
+    int32_t dtype;               /* MARS_DTYPE_F16 or MARS_DTYPE_BF16 */
+    int32_t num_pages;
+    int32_t page_size;
+    int32_t kv_heads;
+    int32_t head_dim;
+    int32_t reserved;            /* 0 */
+    int64_t k_page_stride, k_slot_stride, k_head_stride;
+    int64_t v_page_stride, v_slot_stride, v_head_stride;
+} mars_kv_cache;
+
+/* Rotary positions with n_axes axes.  Pair i < rot_dim / 2 of a head turns by
+ * d_positions[token * n_axes + d_axis[i]] * d_freq[i]; its columns are (i,
+ * i + rot_dim / 2), or (2i, 2i + 1) when interleaved; columns from rot_dim on
+ * are copied.  Text has one axis; an image or video has its tokens' time, row
+ * and column, and d_axis says which pairs each of them turns. */
+typedef struct mars_rope_table {
+    const float*   d_freq;       /* rot_dim / 2 */
+    const int32_t* d_axis;       /* rot_dim / 2, each in [0, n_axes) */
+    int32_t rot_dim;             /* even, <= head_dim and <= 1024 */
+    int32_t n_axes;
+    int32_t interleaved;
+    int32_t reserved;            /* 0 */
+} mars_rope_table;
+
+/* y = the rotation of x (tokens x heads x head_dim of MARS_DTYPE_*, strides in
+ * elements, the columns contiguous; y may be x), computed in fp32 and rounded
+ * once.  inverse != 0 turns back, which is also the gradient: dx = the inverse
+ * rotation of dy.  Runs on the current device; NULL stream: its default
+ * stream. */
+int mars_rope(const mars_rope_table* table, int32_t dtype, const void* d_x, int64_t x_token_stride,
+              int64_t x_head_stride, void* d_y, int64_t y_token_stride, int64_t y_head_stride,
+              int32_t tokens, int32_t heads, int32_t head_dim, const int32_t* d_positions,
+              int32_t inverse, void* stream);
+
+/* One launch for a layer's new tokens: q rotated into d_q_out (may be d_q), k
+ * rotated and v copied into the cache at d_slots[token].  A slot outside the
+ * cache (-1: padding of a fixed-size call) writes neither.  q, k and v are
+ * tokens x heads x head_dim of the cache's dtype and may be slices of one
+ * projection's output.  Runs on the current device; NULL stream: its default
+ * stream. */
+int mars_rope_append(const mars_rope_table* table, const mars_kv_cache* cache, const void* d_q,
+                     int64_t q_token_stride, int64_t q_head_stride, const void* d_k,
+                     int64_t k_token_stride, int64_t k_head_stride, const void* d_v,
+                     int64_t v_token_stride, int64_t v_head_stride, void* d_q_out,
+                     int64_t q_out_token_stride, int64_t q_out_head_stride, int32_t tokens,
+                     int32_t q_heads, const int32_t* d_positions, const int32_t* d_slots, void* stream);
+
 /* Diagnostic: the fused score of every row (same arithmetic as the scan),
  * d_out: N floats, -FLT_MAX for rows rejected by the filter. */
 int mars_debug_fused_scores(const mars_store* s, mars_query_ctx* ctx,
