@@ -176,6 +176,8 @@ _SIGS.update({
     "mars_rope": [_VP, _I32, _VP, _I64, _I64, _VP, _I64, _I64, _I32, _I32, _I32, _VP, _I32, _VP],
     "mars_rope_append": [_VP, _VP, _VP, _I64, _I64, _VP, _I64, _I64, _VP, _I64, _I64, _VP, _I64, _I64, _I32, _I32,
                          _VP, _VP, _VP],
+    "mars_paged_attention": [_VP, _VP, _VP, _I64, _I64, _I32, _I32, _I32, _VP, _VP, _VP, _I32, _VP, _VP, _VP, _VP,
+                             _I64, _I64, _VP, _VP],
 })
 _RESTYPE = {"mars_last_error": C.c_char_p, "mars_status_string": C.c_char_p,
             "mars_abi_version": C.c_int, "mars_query_ctx_stream": C.c_void_p}

@@ -6,6 +6,7 @@ A step of a program that answers with retrieved memories:
     plan = ctx.plan(lens, new_lens, tables, free, count, page_size=64, max_tokens=n)
     for each layer, with q, k, v its new tokens' projections:
         q = rope_append(q, k, v, positions, freq, axis, cache, plan.slots)
+        out = ctx.attention(q, cache, tables, plan.kv_lens, plan.cu_new, max_new=1)
 
 rope is the rotation by itself, for programs that train; its gradient is
 rope(..., inverse=True) of the output's gradient.
@@ -65,6 +66,11 @@ class _Table(C.Structure):
     """mars_rope_table."""
     _fields_ = [("freq", C.c_void_p), ("axis", C.c_void_p), ("rot_dim", C.c_int32), ("n_axes", C.c_int32),
                 ("interleaved", C.c_int32), ("reserved", C.c_int32)]
+
+
+class _Config(C.Structure):
+    """mars_attn_config."""
+    _fields_ = [("scale", C.c_float), ("softcap", C.c_float), ("window", C.c_int32), ("max_new", C.c_int32)]
 
 
 class KvCache:
@@ -184,6 +190,38 @@ class KvContext:
             _ints("free_count", free_count, 1), max_tokens, lens_out.data_ptr(), count_out.data_ptr(),
             cu_new.data_ptr(), slots.data_ptr(), positions.data_ptr(), status.data_ptr(), _stream(stream, kv_lens)))
         return KvPlan(lens_out, cu_new, slots, positions, count_out, status)
+
+    def attention(self, q, cache, tables, kv_lens, cu_new, *, max_new=None, scale=None, softcap=0.0, window=0,
+                  decay=None, prefix_lens=None, out=None, return_lse=False, stream=None):
+        """Attention of q [tokens, q_heads, head_dim], the requests' new tokens back to back (request b's from
+        cu_new[b] to cu_new[b+1], already in the cache), over the pages of tables [B, pages].  kv_lens counts the
+        new tokens.  A row at position i sees key j when j < prefix_lens[b], or j <= i and (window 0 or i - j <
+        window); scores are scale * q.k (scale None: head_dim ** -0.5), capped by softcap * tanh(. / softcap), minus
+        decay[head] * max(0, i - j).  max_new: the most new tokens of one request, if known (it chooses the kernel).
+        Returns out (q's shape and type), with return_lse also the fp32 [tokens, q_heads] log of the scores'
+        exponentials' sum."""
+        qt, qh = _heads("q", q)
+        if q.dtype is not cache.k.dtype or q.device != cache.k.device or q.shape[2] != cache._c.head_dim:
+            raise ValueError("q must have the cache's type, device and columns")
+        B = kv_lens.shape[0]
+        if decay is not None and (decay.dtype is not torch.float32 or not decay.is_cuda or
+                                  not decay.is_contiguous() or decay.shape != (q.shape[1],)):
+            raise ValueError("decay must be a contiguous float32 CUDA tensor of q_heads entries")
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        ot, oh = _heads("out", out, q)
+        if out.shape != q.shape:
+            raise ValueError("out must have q's shape")
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
+        cfg = _Config(q.shape[2] ** -0.5 if scale is None else scale, softcap, window,
+                      q.shape[0] if max_new is None else max_new)
+        _check(lib().mars_paged_attention(
+            self.handle, C.byref(cache._c), q.data_ptr(), qt, qh, q.shape[0], q.shape[1], B,
+            _ints("cu_new", cu_new, B + 1), _ints("kv_lens", kv_lens), _ints("tables", tables, B, 2), tables.shape[1],
+            C.byref(cfg), None if decay is None else decay.data_ptr(),
+            None if prefix_lens is None else _ints("prefix_lens", prefix_lens, B), out.data_ptr(), ot, oh,
+            None if lse is None else lse.data_ptr(), _stream(stream, q)))
+        return (out, lse) if return_lse else out
 
     def close(self):
         if getattr(self, "handle", None):

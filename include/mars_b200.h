@@ -697,6 +697,45 @@ int mars_rope_append(const mars_rope_table* table, const mars_kv_cache* cache, c
                      int64_t q_out_token_stride, int64_t q_out_head_stride, int32_t tokens,
                      int32_t q_heads, const int32_t* d_positions, const int32_t* d_slots, void* stream);
 
+/* Attention of the new tokens of B requests over their pages.  Row r of
+ * request b (token d_cu_new[b] + r of q) stands at position i = d_kv_lens[b]
+ * - (d_cu_new[b+1] - d_cu_new[b]) + r and sees key j < d_kv_lens[b] when
+ *     j < d_prefix_lens[b],  or  j <= i and (window == 0 or i - j < window).
+ * Its score is softcap * tanh(scale * q.k / softcap) (softcap 0: scale * q.k)
+ * minus d_decay[head] * max(0, i - j): the temporal decay of the retrieval in
+ * softmax form, with the distance in tokens as the age.  out = the softmax's
+ * mean of the values; lse (may be NULL) = log of the sum of exp(score), by
+ * which two parts of an attention are joined.  A row that sees nothing gets
+ * out = 0 and lse = -inf.  Query head h reads key head h / (q_heads /
+ * kv_heads).  d_decay and d_prefix_lens may be NULL (none).
+ *
+ * q, out: tokens x q_heads x head_dim of the cache's dtype; lse: tokens x
+ * q_heads fp32.  Tokens from d_cu_new[B] on are left alone.  max_new is the
+ * caller's bound on the new tokens of one request and chooses the kernel: a
+ * request with more is answered rightly, only slower.  Scores, softmax
+ * statistics and the sums are fp32; the softmax's weights are rounded to the
+ * cache's dtype for the product with the values.  What lies in the cache at
+ * or beyond a request's length, or before all its rows' windows, has no
+ * influence, non-finite values included; of the keys below the length, the
+ * values must be finite.  A table entry outside [0, num_pages) reads as zero
+ * keys and values.
+ * Limits: head_dim a multiple of 8 up to 128, page_size a multiple of 8, at
+ * most 128 query heads a key head; all rows on 16-byte boundaries. */
+#define MARS_ATTN_MAX_HEAD_DIM 128
+#define MARS_ATTN_MAX_GROUP 128
+typedef struct mars_attn_config {
+    float   scale;
+    float   softcap;             /* 0: none */
+    int32_t window;              /* 0: none */
+    int32_t max_new;
+} mars_attn_config;
+int mars_paged_attention(mars_kv_ctx* ctx, const mars_kv_cache* cache, const void* d_q,
+                         int64_t q_token_stride, int64_t q_head_stride, int32_t tokens, int32_t q_heads,
+                         int32_t B, const int32_t* d_cu_new, const int32_t* d_kv_lens,
+                         const int32_t* d_tables, int32_t table_pitch, const mars_attn_config* cfg,
+                         const float* d_decay, const int32_t* d_prefix_lens, void* d_out,
+                         int64_t out_token_stride, int64_t out_head_stride, float* d_lse, void* stream);
+
 /* Diagnostic: the fused score of every row (same arithmetic as the scan),
  * d_out: N floats, -FLT_MAX for rows rejected by the filter. */
 int mars_debug_fused_scores(const mars_store* s, mars_query_ctx* ctx,
