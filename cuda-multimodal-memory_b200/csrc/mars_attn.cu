@@ -1,13 +1,17 @@
 // mars_attn.cu -- attention of each request's new tokens over its cache pages.
 // First form: one warp for each (token, query head), one key at a time.
+#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
+#include <mutex>
 #include <string>
 
 #include "mars_attn.cuh"
+#include "mars_attn_mma.cuh"
 #include "mars_kv.h"
 
 using namespace mars;
@@ -77,7 +81,64 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a) {
     if (lane == 0 && a.lse != nullptr) a.lse[w] = l > 0.0f ? m + logf(l) : -INFINITY;
 }
 
+PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    });
+    return fn;
+}
+
 }  // namespace
+
+namespace mars {
+
+int page_box(int page, int tile) {
+    int box = 8;                              // page sizes are multiples of 8
+    while (box * 2 <= tile && page % (box * 2) == 0) box *= 2;
+    return box;
+}
+
+// dimensions: column, token of the page, head, page; out of range reads as 0
+int page_maps(const mars_kv_cache* c, int box, CUtensorMap* k, CUtensorMap* v) {
+    auto enc = get_encode();
+    if (enc == nullptr) return fail(MARS_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+    const cuuint64_t dim[4] = {(cuuint64_t)c->head_dim, (cuuint64_t)c->page_size, (cuuint64_t)c->kv_heads,
+                               (cuuint64_t)c->num_pages};
+    const cuuint32_t shape[4] = {64, (cuuint32_t)box, 1, 1}, unit[4] = {1, 1, 1, 1};
+    const CUtensorMapDataType type =
+        c->dtype == MARS_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const struct { CUtensorMap* map; void* base; int64_t slot, head, page; } side[2] = {
+        {k, c->k, c->k_slot_stride, c->k_head_stride, c->k_page_stride},
+        {v, c->v, c->v_slot_stride, c->v_head_stride, c->v_page_stride}};
+    for (const auto& s : side) {
+        const cuuint64_t stride[3] = {(cuuint64_t)s.slot * 2, (cuuint64_t)s.head * 2, (cuuint64_t)s.page * 2};
+        const CUresult r = enc(s.map, type, 4, s.base, dim, stride, shape, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r != CUDA_SUCCESS)
+            return fail(MARS_ERR_INVALID, "mars_paged_attention: the cache's strides make no tensor map (" +
+                                              std::to_string((int)r) + ")");
+    }
+    return MARS_OK;
+}
+
+int allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    MARS_CUDA_TRY(cudaGetDevice(&dev));
+    const uint64_t bit = 1ull << (dev & 63);
+    if ((done.load(std::memory_order_relaxed) & bit) != 0) return MARS_OK;
+    MARS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(bit);
+    return MARS_OK;
+}
+
+}  // namespace mars
 
 extern "C" int mars_paged_attention(mars_kv_ctx* c, const mars_kv_cache* cache, const void* d_q,
                                     int64_t q_token_stride, int64_t q_head_stride, int32_t tokens, int32_t q_heads,
@@ -121,6 +182,13 @@ extern "C" int mars_paged_attention(mars_kv_ctx* c, const mars_kv_cache* cache, 
     a.scale = cfg->scale; a.cap = cfg->softcap; a.window = cfg->window;
     a.T = tokens; a.B = B; a.hq = q_heads; a.hkv = cache->kv_heads; a.group = q_heads / cache->kv_heads;
     a.D = cache->head_dim; a.page = cache->page_size; a.num_pages = cache->num_pages; a.pitch = table_pitch;
+    AttnWork w{};
+    w.part_o = c->d_part_o; w.part_ml = c->d_part_ml; w.tickets = c->d_tickets + kKvTickets; w.err = c->d_err;
+    w.host_err = c->h_err;
+    if ((int64_t)std::max(cfg->max_new, 1) * a.group <= kShortRows) {
+        MARS_TRY(attn_short(a, w, cache, c->num_sms, st));
+        return kv_end(c, st);
+    }
     const unsigned grid = (unsigned)(((int64_t)tokens * q_heads + 3) / 4);
     if (cache->dtype == MARS_DTYPE_F16) attn_rows_kernel<__half><<<grid, 128, 0, st>>>(a);
     else attn_rows_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(a);

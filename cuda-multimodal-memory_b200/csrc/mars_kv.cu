@@ -21,6 +21,7 @@
 #include <algorithm>
 #include <string>
 
+#include "mars_attn_mma.cuh"
 #include "mars_kv.h"
 
 using namespace mars;
@@ -28,6 +29,14 @@ using namespace mars;
 namespace mars {
 
 int kv_begin(mars_kv_ctx* c, void* stream, cudaStream_t* st) {
+    if (*static_cast<volatile int*>(c->h_err) != 0) {
+        // the kernel that gave up has ended all the same; start the next one clean
+        MARS_CUDA_TRY(cudaEventSynchronize(c->used));
+        MARS_CUDA_TRY(cudaMemsetAsync(c->d_err, 0, sizeof(int), c->last));
+        MARS_CUDA_TRY(cudaEventRecord(c->used, c->last));
+        *c->h_err = 0;
+        return fail(MARS_ERR_TIMEOUT, "an earlier call's bounded wait gave up: its results are not valid");
+    }
     *st = stream != nullptr ? static_cast<cudaStream_t>(stream) : c->stream;
     if (c->any && *st != c->last) {
         cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
@@ -288,23 +297,29 @@ extern "C" int mars_kv_ctx_create(int32_t device, int32_t max_requests, mars_kv_
     if (device < 0 || device >= count) return fail(MARS_ERR_INVALID, "mars_kv_ctx_create: no such device");
     MarsDeviceGuard g(device);
     if (!g.ok) return fail(MARS_ERR_CUDA, "mars_kv_ctx_create: cudaSetDevice failed");
-    cudaDeviceProp prop;
-    MARS_CUDA_TRY(cudaGetDeviceProperties(&prop, device));
-    if (prop.major != 10) return fail(MARS_ERR_NO_DEVICE, "mars_kv_ctx_create: needs an sm_100 device");
+    int major = 0, sms = 0;
+    MARS_CUDA_TRY(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device));
+    MARS_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+    if (major != 10) return fail(MARS_ERR_NO_DEVICE, "mars_kv_ctx_create: needs an sm_100 device");
     mars_kv_ctx* c = new mars_kv_ctx();
     c->device = device;
     c->max_requests = max_requests;
-    c->num_sms = prop.multiProcessorCount;
+    c->num_sms = sms;
     auto build = [&]() -> int {
         MARS_CUDA_TRY(cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking));
         MARS_CUDA_TRY(cudaEventCreateWithFlags(&c->used, cudaEventDisableTiming));
-        MARS_CUDA_TRY(cudaMalloc(&c->d_tickets, kKvTickets * sizeof(unsigned int)));
-        MARS_CUDA_TRY(cudaMemset(c->d_tickets, 0, kKvTickets * sizeof(unsigned int)));
+        const size_t ctas = 2 * (size_t)sms, slots = 2 * ctas, words = kKvTickets + ctas + 1;
+        MARS_CUDA_TRY(cudaMalloc(&c->d_tickets, words * sizeof(unsigned int)));
+        c->d_err = reinterpret_cast<int*>(c->d_tickets + kKvTickets + ctas);
+        MARS_CUDA_TRY(cudaMalloc(&c->d_part_o, slots * kShortRows * kPartCols * sizeof(float)));
+        MARS_CUDA_TRY(cudaMalloc(&c->d_part_ml, slots * kShortRows * sizeof(float2)));
+        MARS_CUDA_TRY(cudaHostAlloc(&c->h_err, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable));
+        *c->h_err = 0;
+        MARS_CUDA_TRY(cudaMemsetAsync(c->d_tickets, 0, words * sizeof(unsigned int), c->stream));
         // the largest context's: the attribute is the device's, not the context's
         MARS_CUDA_TRY(cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            (3 * MARS_KV_MAX_REQUESTS + 2) * (int)sizeof(int32_t)));
-        // other streams do not wait for the legacy stream's memset
-        MARS_CUDA_TRY(cudaDeviceSynchronize());
+        MARS_CUDA_TRY(cudaStreamSynchronize(c->stream));
         return MARS_OK;
     };
     const int st = build();
@@ -321,6 +336,9 @@ extern "C" int mars_kv_ctx_destroy(mars_kv_ctx* c) {
     MarsDeviceGuard g(c->device);
     if (c->any) cudaEventSynchronize(c->used);
     if (c->d_tickets != nullptr) cudaFree(c->d_tickets);
+    if (c->d_part_o != nullptr) cudaFree(c->d_part_o);
+    if (c->d_part_ml != nullptr) cudaFree(c->d_part_ml);
+    if (c->h_err != nullptr) cudaFreeHost(c->h_err);
     if (c->used != nullptr) cudaEventDestroy(c->used);
     if (c->stream != nullptr) cudaStreamDestroy(c->stream);
     delete c;

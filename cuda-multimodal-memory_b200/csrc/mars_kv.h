@@ -16,8 +16,17 @@ struct mars_kv_ctx {
     cudaStream_t stream = nullptr;
 
     // Arrival counters (kTicket*), zero between calls: a call's last block
-    // puts back the one it used.
+    // puts back the one it used.  First kKvTickets, then one for each CTA of an
+    // attention kernel.
     unsigned int* d_tickets = nullptr;
+
+    // Attention: parts of units that several CTAs share (mars_attn_short.cu),
+    // and the word that a bounded wait which gave up sets, on the device for
+    // the kernel's other warps and in mapped host memory for the next call.
+    float* d_part_o = nullptr;
+    float2* d_part_ml = nullptr;
+    int* d_err = nullptr;
+    int* h_err = nullptr;
 
     // The working memory above holds one call at a time.  `used` is recorded
     // after every call outside a capture; a call on another stream waits for it.
