@@ -1,8 +1,6 @@
-// mars_attn.cu -- attention of each request's new tokens over its cache pages.
-// First form: one warp for each (token, query head), one key at a time.
+// mars_attn.cu -- attention of each request's new tokens over its cache pages:
+// the entry point, its checks, the choice of the kernel and the tensor maps.
 #include <cudaTypedefs.h>
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -17,69 +15,6 @@
 using namespace mars;
 
 namespace {
-
-template <typename T> __device__ __forceinline__ float to_f(T x);
-template <> __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
-template <> __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T> __device__ __forceinline__ T from_f(float x);
-template <> __device__ __forceinline__ __half from_f(float x) { return __float2half_rn(x); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat16_rn(x); }
-
-template <typename T>
-__global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a) {
-    const int lane = threadIdx.x & 31;
-    const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (w >= (int64_t)a.T * a.hq) return;
-    const int t = (int)(w / a.hq), h = (int)(w % a.hq);
-    int lo = 0, hi = a.B;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.cu_new[mid] <= t) lo = mid; else hi = mid;
-    }
-    const Request r = load_request(a, lo);
-    if (t < r.first || t >= r.first + r.rows) return;
-    int low, high;
-    row_range(a, r, t - r.first, t - r.first + 1, &low, &high);
-    const int pos = r.len - r.rows + (t - r.first);
-    const T* q = reinterpret_cast<const T*>(a.q) + t * a.q_tok + h * a.q_head;
-    float qv[4], acc[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        acc[i] = 0.0f;
-        qv[i] = lane + 32 * i < a.D ? to_f(q[lane + 32 * i]) : 0.0f;
-    }
-    float m = -INFINITY, l = 0.0f;
-    const float decay = a.decay != nullptr ? a.decay[h] : 0.0f;
-    for (int j = 0; j < high; ++j) {
-        if (j >= r.prefix && j < low) { j = low - 1; continue; }
-        const int page = a.tables[(int64_t)lo * a.pitch + j / a.page];
-        const bool there = page >= 0 && page < a.num_pages;
-        const T* k = reinterpret_cast<const T*>(a.k) + page * a.k_page + (j % a.page) * a.k_slot + (h / a.group) * a.k_head;
-        const T* v = reinterpret_cast<const T*>(a.v) + page * a.v_page + (j % a.page) * a.v_slot + (h / a.group) * a.v_head;
-        float s = 0.0f, vv[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bool in = there && lane + 32 * i < a.D;
-            vv[i] = in ? to_f(v[lane + 32 * i]) : 0.0f;
-            s += in ? qv[i] * to_f(k[lane + 32 * i]) : 0.0f;
-        }
-#pragma unroll
-        for (int off = 16; off >= 1; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-        s *= a.scale;
-        if (a.cap > 0.0f) s = a.cap * tanh_exp(s / a.cap);
-        s -= decay * (float)max(0, pos - j);
-        const float mm = fmaxf(m, s), keep = __expf(m - mm), p = __expf(s - mm);
-        l = l * keep + p;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = acc[i] * keep + p * vv[i];
-        m = mm;
-    }
-    T* o = reinterpret_cast<T*>(a.out) + t * a.o_tok + h * a.o_head;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (lane + 32 * i < a.D) o[lane + 32 * i] = from_f<T>(l > 0.0f ? acc[i] / l : 0.0f);
-    if (lane == 0 && a.lse != nullptr) a.lse[w] = l > 0.0f ? m + logf(l) : -INFINITY;
-}
 
 PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
@@ -128,6 +63,22 @@ int page_maps(const mars_kv_cache* c, int box, CUtensorMap* k, CUtensorMap* v) {
     return MARS_OK;
 }
 
+// dimensions: column, query head of a key head, key head, token
+int query_map(const AttnArgs& a, int32_t dtype, int tokens, CUtensorMap* q) {
+    auto enc = get_encode();
+    if (enc == nullptr) return fail(MARS_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+    const cuuint64_t dim[4] = {(cuuint64_t)a.D, (cuuint64_t)a.group, (cuuint64_t)a.hkv, (cuuint64_t)a.T};
+    const cuuint64_t stride[3] = {(cuuint64_t)a.q_head * 2, (cuuint64_t)a.q_head * a.group * 2, (cuuint64_t)a.q_tok * 2};
+    const cuuint32_t shape[4] = {64, (cuuint32_t)a.group, 1, (cuuint32_t)tokens}, unit[4] = {1, 1, 1, 1};
+    const CUresult r = enc(q, dtype == MARS_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                           4, const_cast<void*>(a.q), dim, stride, shape, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(MARS_ERR_INVALID, "mars_paged_attention: q's strides make no tensor map (" + std::to_string((int)r) + ")");
+    return MARS_OK;
+}
+
 int allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
     int dev = 0;
     MARS_CUDA_TRY(cudaGetDevice(&dev));
@@ -163,13 +114,21 @@ extern "C" int mars_paged_attention(mars_kv_ctx* c, const mars_kv_cache* cache, 
     if (tokens == 0 || B == 0) return MARS_OK;
     if (d_q == nullptr || d_cu_new == nullptr || d_kv_lens == nullptr || d_tables == nullptr || d_out == nullptr)
         return fail(MARS_ERR_INVALID, fn + ": NULL argument");
+    // the stride of a dimension of one entry says nothing
+    mars_kv_cache kv = *cache;
+    if (q_heads == 1) q_head_stride = out_head_stride = kv.head_dim;
+    if (tokens == 1) q_token_stride = out_token_stride = (int64_t)q_heads * kv.head_dim;
+    if (kv.kv_heads == 1) kv.k_head_stride = kv.v_head_stride = kv.head_dim;
+    if (kv.num_pages == 1) kv.k_page_stride = kv.v_page_stride = kv.head_dim;
+    cache = &kv;
     const uintptr_t bases = reinterpret_cast<uintptr_t>(d_q) | reinterpret_cast<uintptr_t>(d_out) |
                             reinterpret_cast<uintptr_t>(cache->k) | reinterpret_cast<uintptr_t>(cache->v);
     const int64_t strides = q_token_stride | q_head_stride | out_token_stride | out_head_stride | cache->k_page_stride |
                             cache->k_slot_stride | cache->k_head_stride | cache->v_page_stride | cache->v_slot_stride |
                             cache->v_head_stride;
-    if ((bases & 15) != 0 || strides % 8 != 0)
-        return fail(MARS_ERR_INVALID, fn + ": q, out, k and v must start on 16 bytes and have strides of multiples of 16 bytes");
+    if ((bases & 15) != 0 || strides % 8 != 0 || strides < 0)
+        return fail(MARS_ERR_INVALID,
+                    fn + ": q, out, k and v must start on 16 bytes and have strides of multiples of 16 bytes, not negative");
     MarsDeviceGuard g(c->device);
     cudaStream_t st;
     MARS_TRY(kv_begin(c, stream, &st));
@@ -184,14 +143,11 @@ extern "C" int mars_paged_attention(mars_kv_ctx* c, const mars_kv_cache* cache, 
     a.D = cache->head_dim; a.page = cache->page_size; a.num_pages = cache->num_pages; a.pitch = table_pitch;
     AttnWork w{};
     w.part_o = c->d_part_o; w.part_ml = c->d_part_ml; w.tickets = c->d_tickets + kKvTickets; w.err = c->d_err;
-    w.host_err = c->h_err;
+    w.host_err = c->h_err; w.chunk_o = c->d_chunk_o; w.chunk_ml = c->d_chunk_ml; w.starts = c->d_starts;
     if ((int64_t)std::max(cfg->max_new, 1) * a.group <= kShortRows) {
         MARS_TRY(attn_short(a, w, cache, c->num_sms, st));
         return kv_end(c, st);
     }
-    const unsigned grid = (unsigned)(((int64_t)tokens * q_heads + 3) / 4);
-    if (cache->dtype == MARS_DTYPE_F16) attn_rows_kernel<__half><<<grid, 128, 0, st>>>(a);
-    else attn_rows_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(a);
-    MARS_CUDA_TRY(cudaGetLastError());
+    MARS_TRY(attn_chunk(a, w, cache, c->num_sms, st));
     return kv_end(c, st);
 }

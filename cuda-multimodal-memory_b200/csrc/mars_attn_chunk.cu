@@ -1,0 +1,647 @@
+// mars_attn_chunk.cu -- attention over the paged cache for chunks and whole
+// prompts, on the 5th-generation tensor cores.
+//
+// A unit is 256 rows of one key head (two tiles of 128: tokens x the query
+// heads that share the key head, so one read of keys and values serves them
+// all) against the 128-key tiles that any of its rows sees.  Scores S = Q K^T
+// go to TMEM, a warpgroup for each of the two row tiles turns them into
+// weights P (one thread a row: no shuffles), writes P over S as the second
+// product's operand, and O += P V stays in TMEM for the whole unit:
+//
+//    TMEM columns   [0,128) S0/P0   [128,256) S1/P1   [256,384) O0   [384,512) O1
+//
+// While one warpgroup exponentiates, the tensor cores work for the other.
+// The running maximum that P is scaled by follows the true one only when it
+// is 2^8 behind: P stays below 2^8 (harmless in fp32 sums and in the type's
+// relative precision), and O is rescaled a few times a unit instead of at
+// every tile.  Sums, maxima and O are fp32; P is rounded to the cache's type
+// because the product takes both operands of one type.
+//
+// Roles of a CTA (one on each SM): warp 0 loads by TMA (a lane for each box of
+// a page), warp 1 issues the products, warp 2 zeroes the values of keys that
+// no row sees (they may be anything, and 0 x NaN is NaN), warps 4-7 and 8-11
+// are the two softmax warpgroups.
+//
+// Work is shared as in mars_attn_short.cu: the units' tiles in one sequence,
+// an equal share for each CTA.  A one-block kernel before it finds the shares
+// (prompts have thousands of units), a kernel after it joins cut units.
+//
+// Bound: the tensor cores and the exponentials, which are even here: 128 x 128
+// scores take 1,024 cycles of products at D = 128 and 1,024 of ex2.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <type_traits>
+
+#include "mars_attn.cuh"
+#include "mars_attn_mma.cuh"
+#include "mars_kv.h"
+#include "mars_sm100.cuh"
+
+using namespace mars;
+using namespace mars::sm100;
+
+namespace {
+
+constexpr int kTile = 128;                      // keys
+constexpr int kRows = 128;                      // rows of one of the two tiles
+constexpr int kThreads = 384;
+constexpr int kUnitCost = 1;                    // a unit's start and end, in tiles
+constexpr float kSlack = 8.0f;                  // how far (log 2) the maximum in use may lag
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int kPanels> struct Layout {
+    static constexpr int kPanel = kTile * 128;                    // bytes: 128 rows x 64 columns
+    static constexpr int kQ = 2 * kPanels * kPanel;
+    static constexpr int kSlot = kPanels * kPanel;                // one tile of keys or of values
+    static constexpr int kSlots = kPanels == 2 ? 5 : 10;
+    static constexpr int kSmem = 1024 + kQ + kSlots * kSlot;
+};
+
+struct Unit {
+    int row0, rows;               // tokens
+    int nq;                       // row tiles: 1 or 2
+    int n1, s2, tiles;            // tiles of the prefix; first tile of the rest; in all
+    int tiles0;                   // tiles that the first row tile sees, from the front
+    int low, high;
+};
+
+__device__ __forceinline__ Unit make_unit(const AttnArgs& a, const Request& r, int qt, int per) {
+    Unit u;
+    u.row0 = qt * 2 * per;
+    u.rows = min(2 * per, r.rows - u.row0);
+    u.nq = u.rows > per ? 2 : 1;
+    row_range(a, r, u.row0, u.row0 + u.rows, &u.low, &u.high);
+    u.n1 = (r.prefix + kTile - 1) / kTile;
+    u.s2 = max(u.n1, u.low / kTile);
+    u.tiles = u.n1 + max(0, (u.high + kTile - 1) / kTile - u.s2);
+    int low0, high0;
+    row_range(a, r, u.row0, u.row0 + min(per, u.rows), &low0, &high0);
+    u.tiles0 = u.n1 + max(0, (high0 + kTile - 1) / kTile - u.s2);
+    return u;
+}
+
+__device__ __forceinline__ int key_of(const Unit& u, int t) { return (t < u.n1 ? t : u.s2 + t - u.n1) * kTile; }
+
+// ---- shares -----------------------------------------------------------------
+
+constexpr int kPlanThreads = 1024;
+
+__device__ long long plan_scan(long long v, long long* total) {
+    __shared__ long long s_sum[kPlanThreads / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long inc = v;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const long long o = __shfl_up_sync(0xffffffffu, inc, off);
+        if (lane >= off) inc += o;
+    }
+    __syncthreads();
+    if (lane == 31) s_sum[warp] = inc;
+    __syncthreads();
+    long long before = 0, all = 0;
+    for (int i = 0; i < kPlanThreads / 32; ++i) {
+        if (i < warp) before += s_sum[i];
+        all += s_sum[i];
+    }
+    *total = all;
+    return before + inc - v;
+}
+
+// starts[i]: where CTA i's share begins; starts[ctas]: the end.
+__global__ void __launch_bounds__(kPlanThreads) attn_chunk_plan_kernel(const AttnArgs a, ChunkStart* starts, int ctas) {
+    extern __shared__ int s_units[];              // B: units (of one head) before request b
+    const int per = kRows / a.group;
+    const int each = (a.B + kPlanThreads - 1) / kPlanThreads;
+    const int b0 = min(a.B, (int)threadIdx.x * each), b1 = min(a.B, b0 + each);
+    long long mine = 0, units;
+    for (int b = b0; b < b1; ++b) mine += (load_request(a, b).rows + 2 * per - 1) / (2 * per);
+    long long at = plan_scan(mine, &units);
+    for (int b = b0; b < b1; ++b) {
+        s_units[b] = (int)at;
+        at += (load_request(a, b).rows + 2 * per - 1) / (2 * per);
+    }
+    __syncthreads();
+    const int n = (int)units, chunk = (n + kPlanThreads - 1) / kPlanThreads;
+    const int u0 = min(n, (int)threadIdx.x * chunk), u1 = min(n, u0 + chunk);
+    int first = 0;
+    if (u0 < u1) {                                // the request of unit u0: the last with s_units[b] <= u0
+        int hi = a.B;
+        while (hi - first > 1) {
+            const int mid = (first + hi) >> 1;
+            if (s_units[mid] <= u0) first = mid; else hi = mid;
+        }
+    }
+    long long cost = 0, total;
+    int b = first;
+    Request r{};
+    if (u0 < u1) r = load_request(a, b);
+    for (int u = u0; u < u1; ++u) {
+        while (u >= s_units[b] + (r.rows + 2 * per - 1) / (2 * per)) r = load_request(a, ++b);
+        cost += (long long)(max(1, make_unit(a, r, u - s_units[b], per).tiles) + kUnitCost) * a.hkv;
+    }
+    long long x = plan_scan(cost, &total);
+    const long long share = max((total + ctas - 1) / ctas, (long long)(2 + kUnitCost));
+    b = first;
+    if (u0 < u1) r = load_request(a, b);
+    for (int u = u0; u < u1; ++u) {
+        while (u >= s_units[b] + (r.rows + 2 * per - 1) / (2 * per)) r = load_request(a, ++b);
+        const int qt = u - s_units[b], tiles = make_unit(a, r, qt, per).tiles, c = max(1, tiles) + kUnitCost;
+        // shares that begin inside this unit's heads
+        for (long long i = (x + share - 1) / share; i < ctas && i * share < x + (long long)c * a.hkv; ++i) {
+            const long long in = i * share - x;
+            starts[i] = ChunkStart{b, qt, (int)(in / c), min(max((int)(in % c) - kUnitCost, 0), max(tiles - 1, 0))};
+        }
+        x += (long long)c * a.hkv;
+    }
+    for (long long i = threadIdx.x; i <= ctas; i += kPlanThreads)
+        if (i == ctas || i * share >= total) starts[i] = ChunkStart{a.B, 0, 0, 0};
+}
+
+// ---- the kernel -------------------------------------------------------------
+
+// A share's pieces, walked alike by every role.
+struct Walk {
+    ChunkStart cur, stop;
+    Request r;
+    Unit u;
+    int begin, end;               // tiles of the unit
+    int count[2];                 // of them, those that each row tile sees
+
+    __device__ __forceinline__ void set(const AttnArgs& a, int per) {
+        u = make_unit(a, r, cur.qt, per);
+        begin = cur.tile;
+        end = u.tiles;
+        if (cur.b == stop.b && cur.qt == stop.qt && cur.h == stop.h) end = stop.tile;
+        const int n = end - begin;
+        count[0] = u.nq == 2 ? max(0, min(u.tiles0 - begin, n)) : n;
+        count[1] = u.nq == 2 ? n : 0;
+    }
+    __device__ __forceinline__ bool start(const AttnArgs& a, const ChunkStart* starts, int per) {
+        cur = starts[blockIdx.x];
+        stop = starts[blockIdx.x + 1];
+        if (done()) return false;
+        r = load_request(a, cur.b);
+        set(a, per);
+        return true;
+    }
+    __device__ __forceinline__ bool done() const {
+        return cur.b == stop.b && cur.qt == stop.qt && cur.h == stop.h && cur.tile == stop.tile;
+    }
+    __device__ __forceinline__ bool next(const AttnArgs& a, int per) {
+        if (cur.b == stop.b && cur.qt == stop.qt && cur.h == stop.h) return false;
+        cur.tile = 0;
+        if (++cur.h == a.hkv) {
+            cur.h = 0;
+            if (++cur.qt * 2 * per >= r.rows) {
+                cur.qt = 0;
+                do {
+                    if (++cur.b >= a.B) return false;
+                    r = load_request(a, cur.b);
+                } while (r.rows == 0);
+            }
+        }
+        if (done()) return false;
+        set(a, per);
+        return true;
+    }
+};
+
+template <typename T, int kPanels>
+__global__ void __launch_bounds__(kThreads, 1)
+attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, const __grid_constant__ CUtensorMap map_q,
+                  const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+    using L = Layout<kPanels>;
+    extern __shared__ uint8_t s_raw[];
+    uint8_t* s_q = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* s_kv = s_q + L::kQ;
+    __shared__ uint64_t s_qfull, s_qempty, s_full[L::kSlots], s_ready[L::kSlots], s_empty[L::kSlots];
+    __shared__ uint64_t s_sfull[2], s_pfull[2], s_ofull[2], s_drain;
+    __shared__ uint32_t s_tmem;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int per = kRows / a.group;              // tokens of a row tile
+    const int ksteps = (a.D + 15) / 16;
+
+    if (tid == 0) {
+        mbar_init(&s_qfull, 1);
+        mbar_init(&s_qempty, 1);
+        for (int i = 0; i < L::kSlots; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&s_ready[i], 1);
+            mbar_init(&s_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_sfull[i], 1);
+            mbar_init(&s_pfull[i], 4);
+            mbar_init(&s_ofull[i], 1);
+        }
+        mbar_init(&s_drain, 1);
+        fence_mbar_init();
+        prefetch_tmap(&map_q);
+        prefetch_tmap(&map_k);
+        prefetch_tmap(&map_v);
+    }
+    if (warp == 1) {
+        tmem_alloc(&s_tmem, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+
+    // registers: 128 x 80 + 256 x 208 of the 384 x 168 at launch
+    bool ok = true;
+    if (warp < 4) {
+        set_max_regs<80, false>();
+        Walk k;
+        bool more = k.start(a, starts, per);
+        if (warp == 0) {
+            // ---- loads -------------------------------------------------------------
+            const int boxes = kTile / w.box;
+            const bool on = lane < boxes * kPanels;
+            const int panel = lane / boxes, at = (lane % boxes) * w.box;
+            int slot_no = 0, q_no = 0;
+            for (; more && ok; more = k.next(a, per)) {
+                if (k.begin == k.end) continue;       // nothing visible: no tile, no query
+                if (q_no > 0 && !__all_sync(0xffffffffu, mbar_wait(&s_qempty, (q_no - 1) & 1, w.err, 1))) { ok = false; break; }
+                ++q_no;
+                if (lane == 0) mbar_arrive_expect_tx(&s_qfull, k.u.nq * kPanels * per * a.group * 128);
+                __syncwarp();
+                if (lane < k.u.nq * kPanels)
+                    tma_load_4d(s_q + lane * L::kPanel, &map_q, &s_qfull, (lane % kPanels) * 64, 0, k.cur.h,
+                                k.r.first + k.u.row0 + (lane / kPanels) * per);
+                const int32_t* table = a.tables + (int64_t)k.cur.b * a.pitch;
+                auto page_of = [&](int t) {           // of this lane's box; num_pages reads as 0
+                    const int key = key_of(k.u, t) + at;
+                    int page = a.num_pages;
+                    if (on && key < k.r.len) {
+                        page = table[key / a.page];
+                        if (page < 0 || page >= a.num_pages) page = a.num_pages;
+                    }
+                    return page;
+                };
+                int page = page_of(k.begin);
+                for (int t = k.begin; t < k.end && ok; ++t) {
+                    const int off = (key_of(k.u, t) + at) % a.page, now = page;
+    #pragma unroll
+                    for (int side = 0; side < 2; ++side, ++slot_no) {
+                        const int slot = slot_no % L::kSlots, phase = (slot_no / L::kSlots) & 1;
+                        if (slot_no >= L::kSlots && !__all_sync(0xffffffffu, mbar_wait(&s_empty[slot], phase ^ 1, w.err, 2))) {
+                            ok = false;
+                            break;
+                        }
+                        if (lane == 0) mbar_arrive_expect_tx(&s_full[slot], L::kSlot);
+                        __syncwarp();
+                        if (on)
+                            tma_load_4d(s_kv + slot * L::kSlot + panel * L::kPanel + at * 128, side == 0 ? &map_k : &map_v,
+                                        &s_full[slot], panel * 64, off, k.cur.h, now);
+                        if (side == 0 && t + 1 < k.end) page = page_of(t + 1);
+                    }
+                }
+            }
+            // no copy may be in flight when the CTA ends
+            for (int i = max(0, slot_no - L::kSlots); i < slot_no; ++i)
+                mbar_wait_drain(&s_full[i % L::kSlots], (i / L::kSlots) & 1, w.err, 3);
+            if (q_no > 0) mbar_wait_drain(&s_qfull, (q_no - 1) & 1, w.err, 3);
+        } else if (warp == 1) {
+            // ---- products ------------------------------------------------------------
+            const uint32_t bf = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
+            const uint32_t idesc_s = idesc_f16(kRows, kTile) | bf;
+            const uint32_t idesc_o = idesc_f16(kRows, ksteps * 16) | bf | (1u << 16);      // B: columns contiguous
+            const uint32_t q0 = smem_u32(s_q), kv0 = smem_u32(s_kv);
+            int slot_no = 0, pieces = 0, pcount[2] = {0, 0};
+            auto scores = [&](int t, int slot) {      // S_t = Q_t K^T
+                if (lane == 0) {
+                    for (int ks = 0; ks < ksteps; ++ks) {
+                        const uint32_t off = (ks >> 2) * L::kPanel + (ks & 3) * 32;
+                        mma_f16(tmem + t * 128, smem_desc_sw128(q0 + t * kPanels * L::kPanel + off),
+                                smem_desc_sw128(kv0 + slot * L::kSlot + off), idesc_s, ks > 0);
+                    }
+                    mma_commit(&s_sfull[t]);
+                }
+            };
+            auto wait = [&](uint64_t* bar, int phase, int code) {
+                ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, w.err, code));
+                return ok;
+            };
+            for (; more && ok; more = k.next(a, per)) {
+                const int n = k.end - k.begin;
+                if (n == 0) continue;
+                if (!wait(&s_qfull, pieces, 4)) break;
+                if (!wait(&s_full[slot_no % L::kSlots], slot_no / L::kSlots, 5)) break;
+                tc_fence_after();
+                for (int t = 0; t < 2; ++t)
+                    if (k.count[t] > 0) scores(t, slot_no % L::kSlots);
+                if (lane == 0) {
+                    mma_commit(&s_empty[slot_no % L::kSlots]);
+                    if (n == 1) mma_commit(&s_qempty);
+                }
+                for (int j = 0; j < n && ok; ++j) {
+                    const int v_no = slot_no + 1, k_no = slot_no + 2;
+                    if (!wait(&s_full[v_no % L::kSlots], v_no / L::kSlots, 6)) break;
+                    if (!wait(&s_ready[(v_no >> 1) % L::kSlots], (v_no >> 1) / L::kSlots, 6)) break;
+                    if (j + 1 < n && !wait(&s_full[k_no % L::kSlots], k_no / L::kSlots, 7)) break;
+                    const uint32_t v = kv0 + (v_no % L::kSlots) * L::kSlot;
+                    for (int t = 0; t < 2 && ok; ++t) {
+                        if (j < k.count[t]) {
+                            if (!wait(&s_pfull[t], pcount[t], 8)) break;
+                            ++pcount[t];
+                            tc_fence_after();
+                            if (lane == 0) {
+                                // O_t (+)= P_t V: 16 keys a step, 8 columns of P, 2,048 B of V
+                                for (int ks = 0; ks < kTile / 16; ++ks)
+                                    mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8,
+                                               smem_desc_mn_sw128(v + ks * 2048, L::kPanel), idesc_o, j > 0 || ks > 0);
+                                if (j + 1 == k.count[t]) mma_commit(&s_ofull[t]);
+                            }
+                            __syncwarp();
+                            if (j + 1 < k.count[t]) scores(t, k_no % L::kSlots);
+                        }
+                    }
+                    if (!ok) break;
+                    if (lane == 0) {
+                        mma_commit(&s_empty[v_no % L::kSlots]);
+                        if (j + 1 < n) mma_commit(&s_empty[k_no % L::kSlots]);
+                        if (j + 2 == n) mma_commit(&s_qempty);
+                    }
+                    slot_no += 2;
+                }
+                ++pieces;
+            }
+            if (lane == 0) {
+                mma_commit(&s_drain);                 // no product may be in flight when TMEM is freed
+                mbar_wait_drain(&s_drain, 0, w.err, 9);
+            }
+            __syncwarp();
+        } else if (warp == 2) {
+            // ---- values that no row sees ----------------------------------------------
+            int slot_no = 0;
+            for (; more && ok; more = k.next(a, per)) {
+                for (int t = k.begin; t < k.end; ++t, slot_no += 2) {
+                    const int v_no = slot_no + 1, slot = v_no % L::kSlots;
+                    ok = ok && __all_sync(0xffffffffu, mbar_wait(&s_full[slot], (v_no / L::kSlots) & 1, w.err, 10));
+                    if (!ok) break;
+                    const int key0 = key_of(k.u, t);
+                    if (!(key0 + kTile <= k.r.prefix || (key0 >= k.u.low && key0 + kTile <= k.u.high))) {
+                        const uint32_t v = smem_u32(s_kv) + slot * L::kSlot;
+                        for (int i = lane; i < kTile; i += 32) {
+                            const int j = key0 + i;
+                            if (!(j < k.r.prefix || (j >= k.u.low && j < k.u.high)))
+                                for (int c = 0; c < kPanels * 8; ++c)
+                                    st_shared_zero16(v + (c >> 3) * L::kPanel + i * 128 + (c & 7) * 16);
+                        }
+                        fence_proxy_async();
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s_ready[(v_no >> 1) % L::kSlots]);      // by value tile: a slot may hold keys next
+                }
+            }
+        }
+    } else {
+        // ---- softmax: warpgroup t, a thread for each row ------------------------------
+        set_max_regs<208, true>();
+        Walk k;
+        bool more = k.start(a, starts, per);
+        const int t = (warp - 4) >> 2, row = tid - 128 - t * 128;
+        const uint32_t tm_s = tmem + ((uint32_t)(warp & 3) << 21) + t * 128;      // lanes of this warp
+        const uint32_t tm_o = tm_s + 256;
+        const bool shaped = a.cap > 0.0f || a.decay != nullptr || !(a.scale > 0.0f);
+        int scount = 0, ocount = 0;
+        for (; more && ok; more = k.next(a, per)) {
+            if (t >= k.u.nq) continue;
+            const int n = k.count[t];
+            const int tok0 = k.u.row0 + t * per, toks = min(per, k.u.rows - t * per);
+            const int tok = tok0 + row / a.group, head = k.cur.h * a.group + row % a.group;
+            const bool valid = row < toks * a.group;
+            const int pos = k.r.len - k.r.rows + tok;
+            const int hi = valid ? min(k.r.len, pos + 1) : 0, pre = valid ? k.r.prefix : 0;
+            const int lo = a.window > 0 ? pos - a.window + 1 : 0;
+            const float decay = valid && a.decay != nullptr ? a.decay[head] * kLog2e : 0.0f;
+            // keys that all rows of the tile see, besides the prefix
+            const int first_pos = k.r.len - k.r.rows + tok0;
+            const int all_hi = min(k.r.len, first_pos + 1), all_lo = a.window > 0 ? first_pos + toks - a.window : 0;
+            float m = -INFINITY, l = 0.0f;
+
+            for (int j = 0; j < n; ++j) {
+                ok = ok && __all_sync(0xffffffffu, mbar_wait(&s_sfull[t], scount & 1, w.err, 11));
+                if (!ok) break;
+                ++scount;
+                tc_fence_after();
+                uint32_t sr[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(tm_s + c * 32, sr[c]);
+                tmem_ld_wait();
+                const int key0 = key_of(k.u, k.begin + j);
+                float f = a.scale * kLog2e;
+                if (shaped) {
+                    // the score in units of log 2 itself
+                    const float in = a.cap > 0.0f ? a.scale / a.cap : 0.0f, out = a.cap * kLog2e;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            float x = __uint_as_float(sr[c][i]);
+                            x = a.cap > 0.0f ? out * tanh_exp(x * in) : x * f;
+                            x -= decay * (float)max(0, pos - (key0 + c * 32 + i));
+                            sr[c][i] = __float_as_uint(x);
+                        }
+                    f = 1.0f;
+                }
+                if (!(key0 + kTile <= k.r.prefix || (key0 >= all_lo && key0 + kTile <= all_hi))) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const int x = key0 + c * 32 + i;
+                            if (!(x < pre || (x >= lo && x < hi))) sr[c][i] = 0xff800000u;
+                        }
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(sr[c][i]));
+                top *= f;                          // f > 0
+                if (__any_sync(0xffffffffu, top > m + kSlack)) {      // m = -inf at first
+                    const float to = fmaxf(top, m);
+                    const float keep = to == -INFINITY ? 1.0f : exp2f_fast(m - to);
+                    if (j > 0) {
+                        // O of the tiles before: complete, since S of this one was issued after them
+#pragma unroll
+                        for (int c = 0; c < 2 * kPanels; ++c) {
+                            if (c * 32 < a.D) {
+                                uint32_t o[32];
+                                tmem_ld_32x32b_x32(tm_o + c * 32, o);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+                                tmem_st_32x32b_x32(tm_o + c * 32, o);
+                            }
+                        }
+                    }
+                    l *= keep;
+                    m = to;
+                }
+                const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t p[16];
+                    float part = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float x = exp2f_fast(fmaf(__uint_as_float(sr[c][2 * i]), f, -base));
+                        const float y = exp2f_fast(fmaf(__uint_as_float(sr[c][2 * i + 1]), f, -base));
+                        part += x + y;
+                        p[i] = pack2<T>(x, y);
+                    }
+                    l += part;
+                    tmem_st_32x32b_x16(tm_s + c * 16, p);
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s_pfull[t]);
+            }
+            if (!ok) break;
+
+            // ---- the piece's end -------------------------------------------------
+            if (n > 0) {
+                ok = ok && __all_sync(0xffffffffu, mbar_wait(&s_ofull[t], ocount & 1, w.err, 12));
+                if (!ok) break;
+                ++ocount;
+                tc_fence_after();
+            }
+            const bool whole = k.begin == 0 && k.end == k.u.tiles;
+            const int slot = 2 * blockIdx.x + (k.begin == 0);
+            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            T* out = reinterpret_cast<T*>(a.out) + (int64_t)(k.r.first + tok) * a.o_tok + (int64_t)head * a.o_head;
+            float* part = w.chunk_o + (int64_t)slot * kPartCols * 2 * kRows + t * kRows + row;
+#pragma unroll
+            for (int c = 0; c < 2 * kPanels; ++c) {
+                if (c * 32 >= a.D) break;
+                uint32_t o[32];
+                if (n > 0) {
+                    tmem_ld_32x32b_x32(tm_o + c * 32, o);
+                    tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = 0;
+                }
+                if (!valid) continue;
+                if (whole) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        if (c * 32 + i < a.D) {
+                            uint32_t p[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                p[e] = pack2<T>(__uint_as_float(o[i + 2 * e]) * inv, __uint_as_float(o[i + 2 * e + 1]) * inv);
+                            *reinterpret_cast<uint4*>(out + c * 32 + i) = make_uint4(p[0], p[1], p[2], p[3]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (c * 32 + i < a.D) part[(int64_t)(c * 32 + i) * 2 * kRows] = __uint_as_float(o[i]);
+                }
+            }
+            if (valid && whole && a.lse != nullptr)
+                a.lse[(int64_t)(k.r.first + tok) * a.hq + head] = l > 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+            if (valid && !whole) w.chunk_ml[slot * 2 * kRows + t * kRows + row] = make_float2(m, l);
+        }
+    }
+    if (!ok && lane == 0) *w.host_err = 1;
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// ---- cut units ----------------------------------------------------------------
+
+// Block (i, group of 32 rows): if share i begins inside a unit and is the first
+// to, joins the unit's parts, in their order: share i-1's end, then i, i+1, ...
+template <typename T>
+__global__ void __launch_bounds__(256) attn_chunk_join_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts,
+                                                              int ctas) {
+    const int i = blockIdx.x + 1;
+    const ChunkStart s = starts[i], p = starts[i - 1];
+    if (s.b >= a.B || s.tile == 0) return;
+    if (p.b == s.b && p.qt == s.qt && p.h == s.h && p.tile > 0) return;      // cut before
+    int parts = 2;
+    while (i + parts - 1 < ctas) {
+        const ChunkStart x = starts[i + parts - 1];
+        if (x.b != s.b || x.qt != s.qt || x.h != s.h || x.tile == 0) break;
+        ++parts;
+    }
+    const int per = kRows / a.group;
+    const Request r = load_request(a, s.b);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int row = blockIdx.y * 32 + lane, t = row / kRows, in = row - t * kRows;
+    const int tok = s.qt * 2 * per + t * per + in / a.group;
+    if (in >= per * a.group || tok >= r.rows) return;
+    auto slot = [&](int n) { return 2 * (i - 1 + n) + (n == 0); };
+    float top = -INFINITY, sum = 0.0f;
+    for (int n = 0; n < parts; ++n) top = fmaxf(top, w.chunk_ml[slot(n) * 2 * kRows + row].x);
+    for (int n = 0; n < parts; ++n) {
+        const float2 ml = w.chunk_ml[slot(n) * 2 * kRows + row];
+        if (ml.x != -INFINITY) sum += ml.y * exp2f_fast(ml.x - top);
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    const int head = s.h * a.group + in % a.group;
+    T* out = reinterpret_cast<T*>(a.out) + (int64_t)(r.first + tok) * a.o_tok + (int64_t)head * a.o_head;
+    for (int d = warp * 8; d < a.D; d += 64) {
+        float v[8] = {};
+        for (int n = 0; n < parts; ++n) {
+            const float pm = w.chunk_ml[slot(n) * 2 * kRows + row].x;
+            const float f = pm == -INFINITY ? 0.0f : exp2f_fast(pm - top);
+            const float* o = w.chunk_o + (int64_t)slot(n) * kPartCols * 2 * kRows + row;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += f * o[(int64_t)(d + e) * 2 * kRows];
+        }
+        *reinterpret_cast<uint4*>(out + d) =
+            make_uint4(pack2<T>(v[0] * inv, v[1] * inv), pack2<T>(v[2] * inv, v[3] * inv),
+                       pack2<T>(v[4] * inv, v[5] * inv), pack2<T>(v[6] * inv, v[7] * inv));
+    }
+    if (warp == 0 && a.lse != nullptr)
+        a.lse[(int64_t)(r.first + tok) * a.hq + head] = sum > 0.0f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+}
+
+template <typename T, int kPanels>
+int launch(const AttnArgs& a, const AttnWork& w, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+           int ctas, cudaStream_t st) {
+    using L = Layout<kPanels>;
+    static std::atomic<uint64_t> done{0};
+    MARS_TRY(allow_smem(reinterpret_cast<const void*>(attn_chunk_kernel<T, kPanels>), L::kSmem, done));
+    attn_chunk_plan_kernel<<<1, kPlanThreads, a.B * sizeof(int), st>>>(a, w.starts, ctas);
+    MARS_CUDA_TRY(cudaGetLastError());
+    attn_chunk_kernel<T, kPanels><<<ctas, kThreads, L::kSmem, st>>>(a, w, w.starts, mq, mk, mv);
+    MARS_CUDA_TRY(cudaGetLastError());
+    if (ctas > 1) {
+        attn_chunk_join_kernel<T><<<dim3(ctas - 1, 2 * kRows / 32), 256, 0, st>>>(a, w, w.starts, ctas);
+        MARS_CUDA_TRY(cudaGetLastError());
+    }
+    return MARS_OK;
+}
+
+}  // namespace
+
+namespace mars {
+
+int attn_chunk(const AttnArgs& a, AttnWork w, const mars_kv_cache* cache, int num_sms, cudaStream_t st) {
+    CUtensorMap mq, mk, mv;
+    w.box = page_box(cache->page_size, kTile);
+    MARS_TRY(page_maps(cache, w.box, &mk, &mv));
+    MARS_TRY(query_map(a, cache->dtype, kRows / a.group, &mq));
+    if (cache->dtype == MARS_DTYPE_F16)
+        return a.D <= 64 ? launch<__half, 1>(a, w, mq, mk, mv, num_sms, st) : launch<__half, 2>(a, w, mq, mk, mv, num_sms, st);
+    return a.D <= 64 ? launch<__nv_bfloat16, 1>(a, w, mq, mk, mv, num_sms, st)
+                     : launch<__nv_bfloat16, 2>(a, w, mq, mk, mv, num_sms, st);
+}
+
+}  // namespace mars

@@ -19,11 +19,20 @@ namespace mars {
 constexpr int kShortRows = 16;            // rows (tokens x query heads of a key head) of a short tile
 constexpr int kPartCols = MARS_ATTN_MAX_HEAD_DIM;
 
+// Where a CTA's share of a chunk call's work begins: key tile `tile` of head h
+// of row tile pair qt of request b.
+struct ChunkStart {
+    int32_t b, qt, h, tile;
+};
+
 // A call's working memory and launch figures.
 struct AttnWork {
     float* part_o;                // parts of split units: slots x rows x kPartCols
     float2* part_ml;              // slots x rows: maximum (log 2 units) and sum
     unsigned int* tickets;        // one for each CTA, zero between calls
+    float* chunk_o;               // chunk kernel: slots x kPartCols x 256 rows
+    float2* chunk_ml;             // slots x 256 rows
+    ChunkStart* starts;           // one for each CTA and the end
     int* err;                     // device word: a bounded wait gave up
     int* host_err;                // the same, where the host sees it
     int box;                      // keys of one TMA box: divides a page and a tile
@@ -91,15 +100,70 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, f
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// D[tmem] (+)= A[tmem] x B[smem], kind::f16: A's rows are lanes, two values a
+// column.
+__device__ __forceinline__ void mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+                                           uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+
+// Descriptor of a 128-byte swizzled operand whose N (or M) index is the
+// contiguous one: rows of 64 values are consecutive K, 8 rows 1,024 bytes;
+// `panel` bytes between blocks of 64 of N.
+__device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t saddr, uint32_t panel) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+    d |= (uint64_t)((panel >> 4) & 0x3FFFu) << 16;
+    d |= (uint64_t)(1024u >> 4) << 32;
+    d |= (uint64_t)1u << 46;
+    d |= (uint64_t)2u << 61;
+    return d;
+}
+
+__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+          "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+          "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Registers of the calling warpgroup from here on.
+template <int kRegs, bool kMore> __device__ __forceinline__ void set_max_regs() {
+    if (kMore) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+
 // Host side (mars_attn.cu).
 // The largest power of two that divides a page and a tile of keys.
 int page_box(int page, int tile);
 // Tensor maps of the pages: box of 64 columns x `box` tokens of one head.
 int page_maps(const mars_kv_cache* cache, int box, CUtensorMap* k, CUtensorMap* v);
+// Tensor map of the queries: box of 64 columns x all heads of one key head x
+// `tokens` tokens.
+int query_map(const AttnArgs& a, int32_t dtype, int tokens, CUtensorMap* q);
 // Allows the kernel `bytes` of dynamic shared memory on the current device
 // (done: the devices where it has been).
 int allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& done);
 
 int attn_short(const AttnArgs& a, AttnWork w, const mars_kv_cache* cache, int num_sms, cudaStream_t st);
+int attn_chunk(const AttnArgs& a, AttnWork w, const mars_kv_cache* cache, int num_sms, cudaStream_t st);
 
 }  // namespace mars

@@ -313,6 +313,10 @@ extern "C" int mars_kv_ctx_create(int32_t device, int32_t max_requests, mars_kv_
         c->d_err = reinterpret_cast<int*>(c->d_tickets + kKvTickets + ctas);
         MARS_CUDA_TRY(cudaMalloc(&c->d_part_o, slots * kShortRows * kPartCols * sizeof(float)));
         MARS_CUDA_TRY(cudaMalloc(&c->d_part_ml, slots * kShortRows * sizeof(float2)));
+        const size_t chunk_rows = 256, chunk_slots = 2 * (size_t)sms;
+        MARS_CUDA_TRY(cudaMalloc(&c->d_chunk_o, chunk_slots * chunk_rows * kPartCols * sizeof(float)));
+        MARS_CUDA_TRY(cudaMalloc(&c->d_chunk_ml, chunk_slots * chunk_rows * sizeof(float2)));
+        MARS_CUDA_TRY(cudaMalloc(&c->d_starts, ((size_t)sms + 1) * sizeof(ChunkStart)));
         MARS_CUDA_TRY(cudaHostAlloc(&c->h_err, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable));
         *c->h_err = 0;
         MARS_CUDA_TRY(cudaMemsetAsync(c->d_tickets, 0, words * sizeof(unsigned int), c->stream));
@@ -338,6 +342,9 @@ extern "C" int mars_kv_ctx_destroy(mars_kv_ctx* c) {
     if (c->d_tickets != nullptr) cudaFree(c->d_tickets);
     if (c->d_part_o != nullptr) cudaFree(c->d_part_o);
     if (c->d_part_ml != nullptr) cudaFree(c->d_part_ml);
+    if (c->d_chunk_o != nullptr) cudaFree(c->d_chunk_o);
+    if (c->d_chunk_ml != nullptr) cudaFree(c->d_chunk_ml);
+    if (c->d_starts != nullptr) cudaFree(c->d_starts);
     if (c->h_err != nullptr) cudaFreeHost(c->h_err);
     if (c->used != nullptr) cudaEventDestroy(c->used);
     if (c->stream != nullptr) cudaStreamDestroy(c->stream);

@@ -9,6 +9,8 @@
 #include "mars_b200.h"
 #include "mars_internal.h"
 
+namespace mars { struct ChunkStart; }
+
 struct mars_kv_ctx {
     int32_t device = 0;
     int32_t max_requests = 0;
@@ -25,6 +27,9 @@ struct mars_kv_ctx {
     // the kernel's other warps and in mapped host memory for the next call.
     float* d_part_o = nullptr;
     float2* d_part_ml = nullptr;
+    float* d_chunk_o = nullptr;         // the same for mars_attn_chunk.cu
+    float2* d_chunk_ml = nullptr;
+    mars::ChunkStart* d_starts = nullptr;
     int* d_err = nullptr;
     int* h_err = nullptr;
 
