@@ -85,6 +85,31 @@ __device__ __forceinline__ Unit make_unit(const AttnArgs& a, const Request& r, i
 
 __device__ __forceinline__ int key_of(const Unit& u, int t) { return (t < u.n1 ? t : u.s2 + t - u.n1) * kTile; }
 
+// The lowest n bits (n < 0: none, n > 31: all).
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
+
+// Two fp32 values in one register pair.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 split(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // ---- shares -----------------------------------------------------------------
 
 constexpr int kPlanThreads = 1024;
@@ -209,7 +234,7 @@ struct Walk {
     }
 };
 
-template <typename T, int kPanels>
+template <typename T, int kPanels, bool kShaped>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, const __grid_constant__ CUtensorMap map_q,
                   const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
@@ -218,7 +243,7 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
     uint8_t* s_q = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* s_kv = s_q + L::kQ;
     __shared__ uint64_t s_qfull, s_qempty, s_full[L::kSlots], s_ready[L::kSlots], s_empty[L::kSlots];
-    __shared__ uint64_t s_sfull[2], s_pfull[2], s_ofull[2], s_drain;
+    __shared__ uint64_t s_sfull[2], s_pfull[2], s_odone[2], s_drain;
     __shared__ uint32_t s_tmem;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int per = kRows / a.group;              // tokens of a row tile
@@ -235,7 +260,7 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_sfull[i], 1);
             mbar_init(&s_pfull[i], 4);
-            mbar_init(&s_ofull[i], 1);
+            mbar_init(&s_odone[i], 1);
         }
         mbar_init(&s_drain, 1);
         fence_mbar_init();
@@ -252,10 +277,10 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
     tc_fence_after();
     const uint32_t tmem = s_tmem;
 
-    // registers: 128 x 80 + 256 x 208 of the 384 x 168 at launch
+    // registers: 128 x 88 + 256 x 208 = the 384 x 168 at launch
     bool ok = true;
     if (warp < 4) {
-        set_max_regs<80, false>();
+        set_max_regs<88, false>();
         Walk k;
         bool more = k.start(a, starts, per);
         if (warp == 0) {
@@ -266,7 +291,7 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
             int slot_no = 0, q_no = 0;
             for (; more && ok; more = k.next(a, per)) {
                 if (k.begin == k.end) continue;       // nothing visible: no tile, no query
-                if (q_no > 0 && !__all_sync(0xffffffffu, mbar_wait(&s_qempty, (q_no - 1) & 1, w.err, 1))) { ok = false; break; }
+                if (q_no > 0 && !warp_wait(&s_qempty, (q_no - 1) & 1, w.err, 1)) { ok = false; break; }
                 ++q_no;
                 if (lane == 0) mbar_arrive_expect_tx(&s_qfull, k.u.nq * kPanels * per * a.group * 128);
                 __syncwarp();
@@ -289,7 +314,7 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
     #pragma unroll
                     for (int side = 0; side < 2; ++side, ++slot_no) {
                         const int slot = slot_no % L::kSlots, phase = (slot_no / L::kSlots) & 1;
-                        if (slot_no >= L::kSlots && !__all_sync(0xffffffffu, mbar_wait(&s_empty[slot], phase ^ 1, w.err, 2))) {
+                        if (slot_no >= L::kSlots && !warp_wait(&s_empty[slot], phase ^ 1, w.err, 2)) {
                             ok = false;
                             break;
                         }
@@ -304,77 +329,116 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
             }
             // no copy may be in flight when the CTA ends
             for (int i = max(0, slot_no - L::kSlots); i < slot_no; ++i)
-                mbar_wait_drain(&s_full[i % L::kSlots], (i / L::kSlots) & 1, w.err, 3);
-            if (q_no > 0) mbar_wait_drain(&s_qfull, (q_no - 1) & 1, w.err, 3);
+                drain_wait(&s_full[i % L::kSlots], (i / L::kSlots) & 1, w.err, 3);
+            if (q_no > 0) drain_wait(&s_qfull, (q_no - 1) & 1, w.err, 3);
         } else if (warp == 1) {
             // ---- products ------------------------------------------------------------
+            // The warp stays together: every lane walks and waits, an elected one issues.
+            // The operands of tcgen05.mma are uniform registers; in code that a single
+            // lane runs by a comparison (lane == 0) they would be copies of that lane's.
             const uint32_t bf = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
             const uint32_t idesc_s = idesc_f16(kRows, kTile) | bf;
             const uint32_t idesc_o = idesc_f16(kRows, ksteps * 16) | bf | (1u << 16);      // B: columns contiguous
-            const uint32_t q0 = smem_u32(s_q), kv0 = smem_u32(s_kv);
-            int slot_no = 0, pieces = 0, pcount[2] = {0, 0};
-            auto scores = [&](int t, int slot) {      // S_t = Q_t K^T
-                if (lane == 0) {
-                    for (int ks = 0; ks < ksteps; ++ks) {
-                        const uint32_t off = (ks >> 2) * L::kPanel + (ks & 3) * 32;
-                        mma_f16(tmem + t * 128, smem_desc_sw128(q0 + t * kPanels * L::kPanel + off),
-                                smem_desc_sw128(kv0 + slot * L::kSlot + off), idesc_s, ks > 0);
-                    }
-                    mma_commit(&s_sfull[t]);
-                }
-            };
+            // An instruction takes the tensor cores 64 cycles, so the descriptors'
+            // arithmetic is an add on their address field (16-byte units).
+            const uint64_t dq = smem_desc_sw128(smem_u32(s_q)), dk = smem_desc_sw128(smem_u32(s_kv));
+            const uint64_t dv = smem_desc_mn_sw128(smem_u32(s_kv), L::kPanel);
+            int slot_no = 0, pieces = 0, pcount0 = 0, pcount1 = 0;
+            int freed = 0, q_freed = 0, s_done0 = 0, s_done1 = 0, o_done0 = 0, o_done1 = 0;      // commits so far
             auto wait = [&](uint64_t* bar, int phase, int code) {
-                ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, w.err, code));
+                ok = ok && warp_wait(bar, phase & 1, w.err, code);
                 return ok;
             };
+            auto scores = [&](int t, int slot, int& done) {      // S_t = Q_t K^T
+                const uint64_t qa = dq + (uint64_t)(t * (kPanels * L::kPanel / 16));
+                const uint64_t kb = dk + (uint64_t)(slot * (L::kSlot / 16));
+#pragma unroll
+                for (int ks = 0; ks < 4 * kPanels; ++ks) {
+                    const uint64_t off = (uint64_t)((ks >> 2) * (L::kPanel / 16) + (ks & 3) * 2);
+                    if (ks < ksteps && elect_one()) mma_f16(tmem + t * 128, qa + off, kb + off, idesc_s, ks > 0 ? 1u : 0u);
+                }
+                if (elect_one()) mma_commit(&s_sfull[t]);
+                ++done;
+            };
+            auto outputs = [&](int t, uint64_t vb, bool add, int& done) {      // O_t (+)= P_t V
+                // 16 keys a step: 8 columns of P, 2,048 bytes of V
+#pragma unroll
+                for (int ks = 0; ks < kTile / 16; ++ks)
+                    if (elect_one())
+                        mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, vb + (uint64_t)(ks * 128), idesc_o,
+                                   add || ks > 0 ? 1u : 0u);
+                if (elect_one()) mma_commit(&s_odone[t]);
+                ++done;
+            };
+            // S_t overwrites P_t.  Products with different accumulators are not ordered
+            // by their issue, so the one that reads P_t has to be done.
+            auto after = [&](int t, int done) { return done == 0 || wait(&s_odone[t], done - 1, 13); };
+            auto free_slot = [&] {                    // the ring's next, once the products so far are done
+                if (elect_one()) mma_commit(&s_empty[freed % L::kSlots]);
+                ++freed;
+            };
+            auto free_query = [&] {
+                if (elect_one()) mma_commit(&s_qempty);
+                ++q_freed;
+            };
             for (; more && ok; more = k.next(a, per)) {
-                const int n = k.end - k.begin;
+                const int n = __shfl_sync(0xffffffffu, k.end - k.begin, 0);
+                const int n0 = __shfl_sync(0xffffffffu, k.count[0], 0), n1 = __shfl_sync(0xffffffffu, k.count[1], 0);
                 if (n == 0) continue;
                 if (!wait(&s_qfull, pieces, 4)) break;
                 if (!wait(&s_full[slot_no % L::kSlots], slot_no / L::kSlots, 5)) break;
+                if (n0 > 0 && !after(0, o_done0)) break;
+                if (n1 > 0 && !after(1, o_done1)) break;
                 tc_fence_after();
-                for (int t = 0; t < 2; ++t)
-                    if (k.count[t] > 0) scores(t, slot_no % L::kSlots);
-                if (lane == 0) {
-                    mma_commit(&s_empty[slot_no % L::kSlots]);
-                    if (n == 1) mma_commit(&s_qempty);
-                }
+                if (n0 > 0) scores(0, slot_no % L::kSlots, s_done0);
+                if (n1 > 0) scores(1, slot_no % L::kSlots, s_done1);
+                free_slot();
+                if (n == 1) free_query();
                 for (int j = 0; j < n && ok; ++j) {
                     const int v_no = slot_no + 1, k_no = slot_no + 2;
                     if (!wait(&s_full[v_no % L::kSlots], v_no / L::kSlots, 6)) break;
                     if (!wait(&s_ready[(v_no >> 1) % L::kSlots], (v_no >> 1) / L::kSlots, 6)) break;
                     if (j + 1 < n && !wait(&s_full[k_no % L::kSlots], k_no / L::kSlots, 7)) break;
-                    const uint32_t v = kv0 + (v_no % L::kSlots) * L::kSlot;
-                    for (int t = 0; t < 2 && ok; ++t) {
-                        if (j < k.count[t]) {
-                            if (!wait(&s_pfull[t], pcount[t], 8)) break;
-                            ++pcount[t];
-                            tc_fence_after();
-                            if (lane == 0) {
-                                // O_t (+)= P_t V: 16 keys a step, 8 columns of P, 2,048 B of V
-                                for (int ks = 0; ks < kTile / 16; ++ks)
-                                    mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8,
-                                               smem_desc_mn_sw128(v + ks * 2048, L::kPanel), idesc_o, j > 0 || ks > 0);
-                                if (j + 1 == k.count[t]) mma_commit(&s_ofull[t]);
-                            }
-                            __syncwarp();
-                            if (j + 1 < k.count[t]) scores(t, k_no % L::kSlots);
+                    const uint64_t vb = dv + (uint64_t)((v_no % L::kSlots) * (L::kSlot / 16));
+                    if (j < n0) {
+                        if (!wait(&s_pfull[0], pcount0, 8)) break;
+                        ++pcount0;
+                        tc_fence_after();
+                        outputs(0, vb, j > 0, o_done0);
+                        if (j + 1 < n0) {
+                            if (!after(0, o_done0)) break;
+                            scores(0, k_no % L::kSlots, s_done0);
                         }
                     }
-                    if (!ok) break;
-                    if (lane == 0) {
-                        mma_commit(&s_empty[v_no % L::kSlots]);
-                        if (j + 1 < n) mma_commit(&s_empty[k_no % L::kSlots]);
-                        if (j + 2 == n) mma_commit(&s_qempty);
+                    if (j < n1) {
+                        if (!wait(&s_pfull[1], pcount1, 8)) break;
+                        ++pcount1;
+                        tc_fence_after();
+                        outputs(1, vb, j > 0, o_done1);
+                        if (j + 1 < n1) {
+                            if (!after(1, o_done1)) break;
+                            scores(1, k_no % L::kSlots, s_done1);
+                        }
                     }
+                    free_slot();
+                    if (j + 1 < n) free_slot();
+                    if (j + 2 == n) free_query();
                     slot_no += 2;
                 }
                 ++pieces;
             }
-            if (lane == 0) {
-                mma_commit(&s_drain);                 // no product may be in flight when TMEM is freed
-                mbar_wait_drain(&s_drain, 0, w.err, 9);
-            }
+            // No product may be in flight when TMEM is freed, and no commit's arrival
+            // when the CTA's shared memory is: the last of each barrier is awaited,
+            // those that no role waits for among them.
+            if (elect_one()) mma_commit(&s_drain);
+            drain_wait(&s_drain, 0, w.err, 9);
+            for (int i = max(0, freed - L::kSlots); i < freed; ++i)
+                drain_wait(&s_empty[i % L::kSlots], (i / L::kSlots) & 1, w.err, 9);
+            if (q_freed > 0) drain_wait(&s_qempty, (q_freed - 1) & 1, w.err, 9);
+            if (s_done0 > 0) drain_wait(&s_sfull[0], (s_done0 - 1) & 1, w.err, 9);
+            if (s_done1 > 0) drain_wait(&s_sfull[1], (s_done1 - 1) & 1, w.err, 9);
+            if (o_done0 > 0) drain_wait(&s_odone[0], (o_done0 - 1) & 1, w.err, 9);
+            if (o_done1 > 0) drain_wait(&s_odone[1], (o_done1 - 1) & 1, w.err, 9);
             __syncwarp();
         } else if (warp == 2) {
             // ---- values that no row sees ----------------------------------------------
@@ -382,7 +446,7 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
             for (; more && ok; more = k.next(a, per)) {
                 for (int t = k.begin; t < k.end; ++t, slot_no += 2) {
                     const int v_no = slot_no + 1, slot = v_no % L::kSlots;
-                    ok = ok && __all_sync(0xffffffffu, mbar_wait(&s_full[slot], (v_no / L::kSlots) & 1, w.err, 10));
+                    ok = ok && warp_wait(&s_full[slot], (v_no / L::kSlots) & 1, w.err, 10);
                     if (!ok) break;
                     const int key0 = key_of(k.u, t);
                     if (!(key0 + kTile <= k.r.prefix || (key0 >= k.u.low && key0 + kTile <= k.u.high))) {
@@ -408,7 +472,6 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
         const int t = (warp - 4) >> 2, row = tid - 128 - t * 128;
         const uint32_t tm_s = tmem + ((uint32_t)(warp & 3) << 21) + t * 128;      // lanes of this warp
         const uint32_t tm_o = tm_s + 256;
-        const bool shaped = a.cap > 0.0f || a.decay != nullptr || !(a.scale > 0.0f);
         int scount = 0, ocount = 0;
         for (; more && ok; more = k.next(a, per)) {
             if (t >= k.u.nq) continue;
@@ -426,79 +489,85 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
             float m = -INFINITY, l = 0.0f;
 
             for (int j = 0; j < n; ++j) {
-                ok = ok && __all_sync(0xffffffffu, mbar_wait(&s_sfull[t], scount & 1, w.err, 11));
+                ok = ok && warp_wait(&s_sfull[t], scount & 1, w.err, 11);
                 if (!ok) break;
                 ++scount;
                 tc_fence_after();
-                uint32_t sr[4][32];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(tm_s + c * 32, sr[c]);
-                tmem_ld_wait();
+                // the row's 128 scores
+                uint32_t sr[2][64];
+                tmem_load(tm_s, sr[0]);
+                tmem_load(tm_s + 64, sr[1]);
                 const int key0 = key_of(k.u, k.begin + j);
-                float f = a.scale * kLog2e;
-                if (shaped) {
-                    // the score in units of log 2 itself
-                    const float in = a.cap > 0.0f ? a.scale / a.cap : 0.0f, out = a.cap * kLog2e;
+                const bool all = key0 + kTile <= k.r.prefix || (key0 >= all_lo && key0 + kTile <= all_hi);
+                float f = a.scale * kLog2e, top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                if (kShaped) f = 1.0f;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                for (int c = 0; c < 4; ++c) {
+                    if (kShaped) {
+                        // the score in units of log 2 itself
+                        if (a.cap > 0.0f) {
+                            const float in = a.scale / a.cap, out = a.cap * kLog2e;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            float x = __uint_as_float(sr[c][i]);
-                            x = a.cap > 0.0f ? out * tanh_exp(x * in) : x * f;
-                            x -= decay * (float)max(0, pos - (key0 + c * 32 + i));
-                            sr[c][i] = __float_as_uint(x);
+                            for (int i = 0; i < 32; ++i) sr[c >> 1][(c & 1) * 32 + i] = __float_as_uint(out * tanh_exp(__uint_as_float(sr[c >> 1][(c & 1) * 32 + i]) * in));
+                        } else {
+                            const float g = a.scale * kLog2e;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) sr[c >> 1][(c & 1) * 32 + i] = __float_as_uint(__uint_as_float(sr[c >> 1][(c & 1) * 32 + i]) * g);
                         }
-                    f = 1.0f;
-                }
-                if (!(key0 + kTile <= k.r.prefix || (key0 >= all_lo && key0 + kTile <= all_hi))) {
+                        if (a.decay != nullptr) {
+                            const float age = (float)(pos - key0 - c * 32);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const int x = key0 + c * 32 + i;
-                            if (!(x < pre || (x >= lo && x < hi))) sr[c][i] = 0xff800000u;
+                            for (int i = 0; i < 32; ++i)
+                                sr[c >> 1][(c & 1) * 32 + i] = __float_as_uint(fmaf(-decay, fmaxf(age - (float)i, 0.0f), __uint_as_float(sr[c >> 1][(c & 1) * 32 + i])));
                         }
+                    }
+                    if (!all) {
+                        const int kb = key0 + c * 32;
+                        const uint32_t seen = low_bits(pre - kb) | (low_bits(hi - kb) & ~low_bits(lo - kb));
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (!((seen >> i) & 1u)) sr[c >> 1][(c & 1) * 32 + i] = 0xff800000u;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2)
+                        top4[(i >> 1) & 3] = fmaxf(top4[(i >> 1) & 3],
+                                                   fmaxf(__uint_as_float(sr[c >> 1][(c & 1) * 32 + i]), __uint_as_float(sr[c >> 1][(c & 1) * 32 + i + 1])));
                 }
-                float top = -INFINITY;
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(sr[c][i]));
-                top *= f;                          // f > 0
+                float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * f;      // f > 0
                 if (__any_sync(0xffffffffu, top > m + kSlack)) {      // m = -inf at first
                     const float to = fmaxf(top, m);
                     const float keep = to == -INFINITY ? 1.0f : exp2f_fast(m - to);
                     if (j > 0) {
                         // O of the tiles before: complete, since S of this one was issued after them
+                        for (int c = 0; c * 32 < a.D; ++c) {
+                            uint32_t o[32];
+                            tmem_load(tm_o + c * 32, o);
 #pragma unroll
-                        for (int c = 0; c < 2 * kPanels; ++c) {
-                            if (c * 32 < a.D) {
-                                uint32_t o[32];
-                                tmem_ld_32x32b_x32(tm_o + c * 32, o);
-                                tmem_ld_wait();
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
-                                tmem_st_32x32b_x32(tm_o + c * 32, o);
-                            }
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+                            tmem_st_32x32b_x32(tm_o + c * 32, o);
                         }
                     }
                     l *= keep;
                     m = to;
                 }
                 const float base = m == -INFINITY ? 0.0f : m;
+                const uint64_t f2 = pair(f, f), base2 = pair(-base, -base);
+                uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     uint32_t p[16];
-                    float part = 0.0f;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float x = exp2f_fast(fmaf(__uint_as_float(sr[c][2 * i]), f, -base));
-                        const float y = exp2f_fast(fmaf(__uint_as_float(sr[c][2 * i + 1]), f, -base));
-                        part += x + y;
+                        const float2 e = split(fma2(pair(__uint_as_float(sr[c >> 1][(c & 1) * 32 + 2 * i]), __uint_as_float(sr[c >> 1][(c & 1) * 32 + 2 * i + 1])), f2, base2));
+                        const float x = exp2f_fast(e.x), y = exp2f_fast(e.y);
+                        sum[i & 3] = add2(sum[i & 3], pair(x, y));
                         p[i] = pack2<T>(x, y);
                     }
-                    l += part;
                     tmem_st_32x32b_x16(tm_s + c * 16, p);
+                }
+                {
+                    const float2 e = split(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
+                    l += e.x + e.y;
                 }
                 tmem_st_wait();
                 tc_fence_before();
@@ -508,10 +577,11 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
             if (!ok) break;
 
             // ---- the piece's end -------------------------------------------------
+            // the product of the last tile (those before it were done when its scores came)
             if (n > 0) {
-                ok = ok && __all_sync(0xffffffffu, mbar_wait(&s_ofull[t], ocount & 1, w.err, 12));
+                ocount += n;
+                ok = ok && warp_wait(&s_odone[t], (ocount - 1) & 1, w.err, 12);
                 if (!ok) break;
-                ++ocount;
                 tc_fence_after();
             }
             const bool whole = k.begin == 0 && k.end == k.u.tiles;
@@ -519,33 +589,36 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
             const float inv = l > 0.0f ? 1.0f / l : 0.0f;
             T* out = reinterpret_cast<T*>(a.out) + (int64_t)(k.r.first + tok) * a.o_tok + (int64_t)head * a.o_head;
             float* part = w.chunk_o + (int64_t)slot * kPartCols * 2 * kRows + t * kRows + row;
+            // TMEM loads are for the whole warp: lanes without a row take part, and all
+            // are together again before the next one.
 #pragma unroll
             for (int c = 0; c < 2 * kPanels; ++c) {
-                if (c * 32 >= a.D) break;
-                uint32_t o[32];
-                if (n > 0) {
-                    tmem_ld_32x32b_x32(tm_o + c * 32, o);
-                    tmem_ld_wait();
-                } else {
+                if (c * 32 < a.D) {
+                    uint32_t o[32];
+                    __syncwarp();
+                    if (n > 0) {
+                        tmem_load(tm_o + c * 32, o);
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = 0;
-                }
-                if (!valid) continue;
-                if (whole) {
-#pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        if (c * 32 + i < a.D) {
-                            uint32_t p[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                p[e] = pack2<T>(__uint_as_float(o[i + 2 * e]) * inv, __uint_as_float(o[i + 2 * e + 1]) * inv);
-                            *reinterpret_cast<uint4*>(out + c * 32 + i) = make_uint4(p[0], p[1], p[2], p[3]);
-                        }
+                        for (int i = 0; i < 32; ++i) o[i] = 0;
                     }
-                } else {
+                    if (valid && whole) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (c * 32 + i < a.D) part[(int64_t)(c * 32 + i) * 2 * kRows] = __uint_as_float(o[i]);
+                        for (int i = 0; i < 32; i += 8) {
+                            if (c * 32 + i < a.D) {
+                                uint32_t p[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    p[e] = pack2<T>(__uint_as_float(o[i + 2 * e]) * inv, __uint_as_float(o[i + 2 * e + 1]) * inv);
+                                *reinterpret_cast<uint4*>(out + c * 32 + i) = make_uint4(p[0], p[1], p[2], p[3]);
+                            }
+                        }
+                    } else if (valid) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (c * 32 + i < a.D) part[(int64_t)(c * 32 + i) * 2 * kRows] = __uint_as_float(o[i]);
+                    }
+                    __syncwarp();
                 }
             }
             if (valid && whole && a.lse != nullptr)
@@ -612,15 +685,15 @@ __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const AttnArgs a, 
         a.lse[(int64_t)(r.first + tok) * a.hq + head] = sum > 0.0f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
 }
 
-template <typename T, int kPanels>
+template <typename T, int kPanels, bool kShaped>
 int launch(const AttnArgs& a, const AttnWork& w, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
            int ctas, cudaStream_t st) {
     using L = Layout<kPanels>;
     static std::atomic<uint64_t> done{0};
-    MARS_TRY(allow_smem(reinterpret_cast<const void*>(attn_chunk_kernel<T, kPanels>), L::kSmem, done));
+    MARS_TRY(allow_smem(reinterpret_cast<const void*>(attn_chunk_kernel<T, kPanels, kShaped>), L::kSmem, done));
     attn_chunk_plan_kernel<<<1, kPlanThreads, a.B * sizeof(int), st>>>(a, w.starts, ctas);
     MARS_CUDA_TRY(cudaGetLastError());
-    attn_chunk_kernel<T, kPanels><<<ctas, kThreads, L::kSmem, st>>>(a, w, w.starts, mq, mk, mv);
+    attn_chunk_kernel<T, kPanels, kShaped><<<ctas, kThreads, L::kSmem, st>>>(a, w, w.starts, mq, mk, mv);
     MARS_CUDA_TRY(cudaGetLastError());
     if (ctas > 1) {
         attn_chunk_join_kernel<T><<<dim3(ctas - 1, 2 * kRows / 32), 256, 0, st>>>(a, w, w.starts, ctas);
@@ -638,10 +711,17 @@ int attn_chunk(const AttnArgs& a, AttnWork w, const mars_kv_cache* cache, int nu
     w.box = page_box(cache->page_size, kTile);
     MARS_TRY(page_maps(cache, w.box, &mk, &mv));
     MARS_TRY(query_map(a, cache->dtype, kRows / a.group, &mq));
-    if (cache->dtype == MARS_DTYPE_F16)
-        return a.D <= 64 ? launch<__half, 1>(a, w, mq, mk, mv, num_sms, st) : launch<__half, 2>(a, w, mq, mk, mv, num_sms, st);
-    return a.D <= 64 ? launch<__nv_bfloat16, 1>(a, w, mq, mk, mv, num_sms, st)
-                     : launch<__nv_bfloat16, 2>(a, w, mq, mk, mv, num_sms, st);
+    // scores that a positive factor alone turns into exponents, or not
+    const bool shaped = a.cap > 0.0f || a.decay != nullptr || !(a.scale > 0.0f);
+    auto go = [&](auto type, auto panels) {
+        using T = decltype(type);
+        return shaped ? launch<T, decltype(panels)::value, true>(a, w, mq, mk, mv, num_sms, st)
+                      : launch<T, decltype(panels)::value, false>(a, w, mq, mk, mv, num_sms, st);
+    };
+    const std::integral_constant<int, 1> one;
+    const std::integral_constant<int, 2> two;
+    if (cache->dtype == MARS_DTYPE_F16) return a.D <= 64 ? go(__half(), one) : go(__half(), two);
+    return a.D <= 64 ? go(__nv_bfloat16(), one) : go(__nv_bfloat16(), two);
 }
 
 }  // namespace mars

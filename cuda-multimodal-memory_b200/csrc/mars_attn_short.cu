@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
             for (int t = cur.tile; t < min(end, u.tiles); ++t) {
                 const int stage = issued % L::kStages, phase = (issued / L::kStages) & 1;
                 if (issued >= L::kStages &&
-                    !__all_sync(0xffffffffu, mbar_wait(&s_empty[stage], phase ^ 1, w.err, 1))) { ok = false; break; }
+                    !warp_wait(&s_empty[stage], phase ^ 1, w.err, 1)) { ok = false; break; }
                 if (lane == 0) mbar_arrive_expect_tx(&s_full[stage], L::kStage);
                 __syncwarp();
                 const int key = (t < u.n1 ? t : u.s2 + t - u.n1) * kTile + at;
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
         }
         // no copy may be in flight when the CTA ends
         for (int i = max(0, issued - L::kStages); i < issued; ++i)
-            mbar_wait_drain(&s_full[i % L::kStages], (i / L::kStages) & 1, w.err, 2);
+            drain_wait(&s_full[i % L::kStages], (i / L::kStages) & 1, w.err, 2);
         if (!ok && lane == 0) *w.host_err = 1;
         return;
     }
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
         for (int t = begin; t < min(end, u.tiles); ++t, ++used) {
             const int stage = used % L::kStages;
             // a wait that gave up: the unit's barriers are still taken, so that no warp is left at one
-            ok = ok && __all_sync(0xffffffffu, mbar_wait(&s_full[stage], (used / L::kStages) & 1, w.err, 3));
+            ok = ok && warp_wait(&s_full[stage], (used / L::kStages) & 1, w.err, 3);
             if (!ok) continue;
             const int key0 = (t < u.n1 ? t : u.s2 + t - u.n1) * kTile + warp * 16;
             const uint32_t sk = smem_u32(ring + stage * L::kStage) + warp * 16 * 128;
