@@ -234,7 +234,21 @@ struct Walk {
     }
 };
 
-template <typename T, int kPanels, bool kShaped>
+// A ring's next slot and the parity of its use.
+template <int kSlots> struct Ring {
+    int slot = 0, phase = 0, rounds = 0;
+    __device__ __forceinline__ void step() {
+        if (++slot == kSlots) {
+            slot = 0;
+            phase ^= 1;
+            ++rounds;
+        }
+    }
+};
+
+// kFull: D = 64 kPanels, every step of the first product.  kShaped: capped
+// scores, a decay or a scale that is not positive.
+template <typename T, int kPanels, bool kFull, bool kShaped>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, const __grid_constant__ CUtensorMap map_q,
                   const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
@@ -339,34 +353,38 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
             const uint32_t bf = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
             const uint32_t idesc_s = idesc_f16(kRows, kTile) | bf;
             const uint32_t idesc_o = idesc_f16(kRows, ksteps * 16) | bf | (1u << 16);      // B: columns contiguous
-            // An instruction takes the tensor cores 64 cycles, so the descriptors'
-            // arithmetic is an add on their address field (16-byte units).
-            const uint64_t dq = smem_desc_sw128(smem_u32(s_q)), dk = smem_desc_sw128(smem_u32(s_kv));
-            const uint64_t dv = smem_desc_mn_sw128(smem_u32(s_kv), L::kPanel);
-            int slot_no = 0, pieces = 0, pcount0 = 0, pcount1 = 0;
-            int freed = 0, q_freed = 0, s_done0 = 0, s_done1 = 0, o_done0 = 0, o_done1 = 0;      // commits so far
+            // An instruction takes the tensor cores 64 cycles, so what leads up to one has
+            // to be short: of a descriptor only the low word changes, by an add on its
+            // address field (16-byte units).
+            const uint32_t q_lo = (smem_u32(s_q) >> 4) | (1u << 16), kv_lo = (smem_u32(s_kv) >> 4) | (1u << 16);
+            const uint32_t v_lo = (smem_u32(s_kv) >> 4) | ((uint32_t)L::kPanel >> 4) << 16;
+            Ring<L::kSlots> ring, vring, freed;       // slots, value tiles, freed slots
+            int pieces = 0, pcount0 = 0, pcount1 = 0;
+            int q_freed = 0, s_done0 = 0, s_done1 = 0, o_done0 = 0, o_done1 = 0;      // commits so far
             auto wait = [&](uint64_t* bar, int phase, int code) {
                 ok = ok && warp_wait(bar, phase & 1, w.err, code);
                 return ok;
             };
             auto scores = [&](int t, int slot, int& done) {      // S_t = Q_t K^T
-                const uint64_t qa = dq + (uint64_t)(t * (kPanels * L::kPanel / 16));
-                const uint64_t kb = dk + (uint64_t)(slot * (L::kSlot / 16));
+                const uint32_t qa = q_lo + (uint32_t)(t * (kPanels * L::kPanel / 16));
+                const uint32_t kb = kv_lo + (uint32_t)(slot * (L::kSlot / 16));
 #pragma unroll
                 for (int ks = 0; ks < 4 * kPanels; ++ks) {
-                    const uint64_t off = (uint64_t)((ks >> 2) * (L::kPanel / 16) + (ks & 3) * 2);
-                    if (ks < ksteps && elect_one()) mma_f16(tmem + t * 128, qa + off, kb + off, idesc_s, ks > 0 ? 1u : 0u);
+                    const uint32_t off = (uint32_t)((ks >> 2) * (L::kPanel / 16) + (ks & 3) * 2);
+                    if (kFull || ks < ksteps) {
+                        if (elect_one()) mma_f16_lo(tmem + t * 128, qa + off, kb + off, idesc_s, ks > 0 ? 1u : 0u);
+                    }
                 }
                 if (elect_one()) mma_commit(&s_sfull[t]);
                 ++done;
             };
-            auto outputs = [&](int t, uint64_t vb, bool add, int& done) {      // O_t (+)= P_t V
+            auto outputs = [&](int t, uint32_t vb, bool add, int& done) {      // O_t (+)= P_t V
                 // 16 keys a step: 8 columns of P, 2,048 bytes of V
 #pragma unroll
                 for (int ks = 0; ks < kTile / 16; ++ks)
                     if (elect_one())
-                        mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, vb + (uint64_t)(ks * 128), idesc_o,
-                                   add || ks > 0 ? 1u : 0u);
+                        mma_f16_ts_lo(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, vb + (uint32_t)(ks * 128), idesc_o,
+                                      add || ks > 0 ? 1u : 0u);
                 if (elect_one()) mma_commit(&s_odone[t]);
                 ++done;
             };
@@ -374,8 +392,8 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
             // by their issue, so the one that reads P_t has to be done.
             auto after = [&](int t, int done) { return done == 0 || wait(&s_odone[t], done - 1, 13); };
             auto free_slot = [&] {                    // the ring's next, once the products so far are done
-                if (elect_one()) mma_commit(&s_empty[freed % L::kSlots]);
-                ++freed;
+                if (elect_one()) mma_commit(&s_empty[freed.slot]);
+                freed.step();
             };
             auto free_query = [&] {
                 if (elect_one()) mma_commit(&s_qempty);
@@ -386,20 +404,23 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
                 const int n0 = __shfl_sync(0xffffffffu, k.count[0], 0), n1 = __shfl_sync(0xffffffffu, k.count[1], 0);
                 if (n == 0) continue;
                 if (!wait(&s_qfull, pieces, 4)) break;
-                if (!wait(&s_full[slot_no % L::kSlots], slot_no / L::kSlots, 5)) break;
+                if (!wait(&s_full[ring.slot], ring.phase, 5)) break;
                 if (n0 > 0 && !after(0, o_done0)) break;
                 if (n1 > 0 && !after(1, o_done1)) break;
                 tc_fence_after();
-                if (n0 > 0) scores(0, slot_no % L::kSlots, s_done0);
-                if (n1 > 0) scores(1, slot_no % L::kSlots, s_done1);
+                if (n0 > 0) scores(0, ring.slot, s_done0);
+                if (n1 > 0) scores(1, ring.slot, s_done1);
                 free_slot();
                 if (n == 1) free_query();
+                ring.step();
                 for (int j = 0; j < n && ok; ++j) {
-                    const int v_no = slot_no + 1, k_no = slot_no + 2;
-                    if (!wait(&s_full[v_no % L::kSlots], v_no / L::kSlots, 6)) break;
-                    if (!wait(&s_ready[(v_no >> 1) % L::kSlots], (v_no >> 1) / L::kSlots, 6)) break;
-                    if (j + 1 < n && !wait(&s_full[k_no % L::kSlots], k_no / L::kSlots, 7)) break;
-                    const uint64_t vb = dv + (uint64_t)((v_no % L::kSlots) * (L::kSlot / 16));
+                    // here: values of tile j; then keys of tile j + 1
+                    if (!wait(&s_full[ring.slot], ring.phase, 6)) break;
+                    if (!wait(&s_ready[vring.slot], vring.phase, 6)) break;
+                    const uint32_t vb = v_lo + (uint32_t)(ring.slot * (L::kSlot / 16));
+                    ring.step();
+                    vring.step();
+                    if (j + 1 < n && !wait(&s_full[ring.slot], ring.phase, 7)) break;
                     if (j < n0) {
                         if (!wait(&s_pfull[0], pcount0, 8)) break;
                         ++pcount0;
@@ -407,7 +428,7 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
                         outputs(0, vb, j > 0, o_done0);
                         if (j + 1 < n0) {
                             if (!after(0, o_done0)) break;
-                            scores(0, k_no % L::kSlots, s_done0);
+                            scores(0, ring.slot, s_done0);
                         }
                     }
                     if (j < n1) {
@@ -417,13 +438,15 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
                         outputs(1, vb, j > 0, o_done1);
                         if (j + 1 < n1) {
                             if (!after(1, o_done1)) break;
-                            scores(1, k_no % L::kSlots, s_done1);
+                            scores(1, ring.slot, s_done1);
                         }
                     }
                     free_slot();
-                    if (j + 1 < n) free_slot();
+                    if (j + 1 < n) {
+                        free_slot();
+                        ring.step();
+                    }
                     if (j + 2 == n) free_query();
-                    slot_no += 2;
                 }
                 ++pieces;
             }
@@ -432,8 +455,10 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
             // those that no role waits for among them.
             if (elect_one()) mma_commit(&s_drain);
             drain_wait(&s_drain, 0, w.err, 9);
-            for (int i = max(0, freed - L::kSlots); i < freed; ++i)
-                drain_wait(&s_empty[i % L::kSlots], (i / L::kSlots) & 1, w.err, 9);
+            for (int i = 0; i < L::kSlots; ++i) {     // slot i's last use: this round's, or the one before
+                const int uses = freed.rounds + (i < freed.slot);
+                if (uses > 0) drain_wait(&s_empty[i], (uses - 1) & 1, w.err, 9);
+            }
             if (q_freed > 0) drain_wait(&s_qempty, (q_freed - 1) & 1, w.err, 9);
             if (s_done0 > 0) drain_wait(&s_sfull[0], (s_done0 - 1) & 1, w.err, 9);
             if (s_done1 > 0) drain_wait(&s_sfull[1], (s_done1 - 1) & 1, w.err, 9);
@@ -442,12 +467,18 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
             __syncwarp();
         } else if (warp == 2) {
             // ---- values that no row sees ----------------------------------------------
-            int slot_no = 0;
+            Ring<L::kSlots> ring, vring;
             for (; more && ok; more = k.next(a, per)) {
-                for (int t = k.begin; t < k.end; ++t, slot_no += 2) {
-                    const int v_no = slot_no + 1, slot = v_no % L::kSlots;
-                    ok = ok && warp_wait(&s_full[slot], (v_no / L::kSlots) & 1, w.err, 10);
+                for (int t = k.begin; t < k.end; ++t) {
+                    // The keys too, in the ring's order: loads land in any order, and a
+                    // parity tells only neighbouring uses of a slot apart.
+                    ok = ok && warp_wait(&s_full[ring.slot], ring.phase, w.err, 10);
                     if (!ok) break;
+                    ring.step();
+                    const int slot = ring.slot;
+                    ok = ok && warp_wait(&s_full[slot], ring.phase, w.err, 10);
+                    if (!ok) break;
+                    ring.step();
                     const int key0 = key_of(k.u, t);
                     if (!(key0 + kTile <= k.r.prefix || (key0 >= k.u.low && key0 + kTile <= k.u.high))) {
                         const uint32_t v = smem_u32(s_kv) + slot * L::kSlot;
@@ -460,7 +491,8 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
                         fence_proxy_async();
                     }
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&s_ready[(v_no >> 1) % L::kSlots]);      // by value tile: a slot may hold keys next
+                    if (lane == 0) mbar_arrive(&s_ready[vring.slot]);      // by value tile: a slot may hold keys next
+                    vring.step();
                 }
             }
         }
@@ -626,7 +658,7 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
             if (valid && !whole) w.chunk_ml[slot * 2 * kRows + t * kRows + row] = make_float2(m, l);
         }
     }
-    if (!ok && lane == 0) *w.host_err = 1;
+    if (!ok && lane == 0) *w.host_err = *(volatile int*)w.err;
     tc_fence_before();
     __syncthreads();
     if (warp == 1) {
@@ -685,15 +717,15 @@ __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const AttnArgs a, 
         a.lse[(int64_t)(r.first + tok) * a.hq + head] = sum > 0.0f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
 }
 
-template <typename T, int kPanels, bool kShaped>
+template <typename T, int kPanels, bool kFull, bool kShaped>
 int launch(const AttnArgs& a, const AttnWork& w, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
            int ctas, cudaStream_t st) {
     using L = Layout<kPanels>;
     static std::atomic<uint64_t> done{0};
-    MARS_TRY(allow_smem(reinterpret_cast<const void*>(attn_chunk_kernel<T, kPanels, kShaped>), L::kSmem, done));
+    MARS_TRY(allow_smem(reinterpret_cast<const void*>(attn_chunk_kernel<T, kPanels, kFull, kShaped>), L::kSmem, done));
     attn_chunk_plan_kernel<<<1, kPlanThreads, a.B * sizeof(int), st>>>(a, w.starts, ctas);
     MARS_CUDA_TRY(cudaGetLastError());
-    attn_chunk_kernel<T, kPanels, kShaped><<<ctas, kThreads, L::kSmem, st>>>(a, w, w.starts, mq, mk, mv);
+    attn_chunk_kernel<T, kPanels, kFull, kShaped><<<ctas, kThreads, L::kSmem, st>>>(a, w, w.starts, mq, mk, mv);
     MARS_CUDA_TRY(cudaGetLastError());
     if (ctas > 1) {
         attn_chunk_join_kernel<T><<<dim3(ctas - 1, 2 * kRows / 32), 256, 0, st>>>(a, w, w.starts, ctas);
@@ -715,8 +747,12 @@ int attn_chunk(const AttnArgs& a, AttnWork w, const mars_kv_cache* cache, int nu
     const bool shaped = a.cap > 0.0f || a.decay != nullptr || !(a.scale > 0.0f);
     auto go = [&](auto type, auto panels) {
         using T = decltype(type);
-        return shaped ? launch<T, decltype(panels)::value, true>(a, w, mq, mk, mv, num_sms, st)
-                      : launch<T, decltype(panels)::value, false>(a, w, mq, mk, mv, num_sms, st);
+        constexpr int kPanels = decltype(panels)::value;
+        if (a.D == 64 * kPanels)
+            return shaped ? launch<T, kPanels, true, true>(a, w, mq, mk, mv, num_sms, st)
+                          : launch<T, kPanels, true, false>(a, w, mq, mk, mv, num_sms, st);
+        return shaped ? launch<T, kPanels, false, true>(a, w, mq, mk, mv, num_sms, st)
+                      : launch<T, kPanels, false, false>(a, w, mq, mk, mv, num_sms, st);
     };
     const std::integral_constant<int, 1> one;
     const std::integral_constant<int, 2> two;

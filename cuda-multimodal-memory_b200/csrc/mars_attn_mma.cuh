@@ -135,28 +135,33 @@ __device__ __forceinline__ bool elect_one() {
     return p != 0;
 }
 
-// D[tmem] (+)= A[tmem] x B[smem], kind::f16: A's rows are lanes, two values a
-// column.
-__device__ __forceinline__ void mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+// Shared-memory descriptors of 128-byte swizzled operands differ in the low
+// word only (address, and the distance of 64-column blocks for the one whose N
+// is the contiguous index); the high word: 1,024 bytes between groups of 8
+// rows, version 1, 128-byte swizzle.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+
+// D[tmem] (+)= A[smem] x B[smem]^T, kind::f16.
+__device__ __forceinline__ void mma_f16_lo(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc,
                                            uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\t"
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
                  "setp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+                 "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}"
+                 ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
                  : "memory");
 }
 
-// Descriptor of a 128-byte swizzled operand whose N (or M) index is the
-// contiguous one: rows of 64 values are consecutive K, 8 rows 1,024 bytes;
-// `panel` bytes between blocks of 64 of N.
-__device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t saddr, uint32_t panel) {
-    uint64_t d = 0;
-    d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
-    d |= (uint64_t)((panel >> 4) & 0x3FFFu) << 16;
-    d |= (uint64_t)(1024u >> 4) << 32;
-    d |= (uint64_t)1u << 46;
-    d |= (uint64_t)2u << 61;
-    return d;
+// D[tmem] (+)= A[tmem] x B[smem], kind::f16: A's rows are lanes, two values a
+// column; B's N index is contiguous, rows of 64 values are consecutive K.
+__device__ __forceinline__ void mma_f16_ts_lo(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t idesc,
+                                              uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "mov.b64 db, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}"
+                 ::"r"(tmem_d), "r"(tmem_a), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
+                 : "memory");
 }
 
 // 32 lanes x N consecutive columns, complete on return: load and wait are one

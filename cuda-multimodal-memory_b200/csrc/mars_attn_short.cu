@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
         // no copy may be in flight when the CTA ends
         for (int i = max(0, issued - L::kStages); i < issued; ++i)
             drain_wait(&s_full[i % L::kStages], (i / L::kStages) & 1, w.err, 2);
-        if (!ok && lane == 0) *w.host_err = 1;
+        if (!ok && lane == 0) *w.host_err = *(volatile int*)w.err;
         return;
     }
 
@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
             }
         }
     }
-    if (!ok && lane == 0) *w.host_err = 1;
+    if (!ok && lane == 0) *w.host_err = *(volatile int*)w.err;
 }
 
 template <typename T, int kPanels>

@@ -34,8 +34,10 @@ int kv_begin(mars_kv_ctx* c, void* stream, cudaStream_t* st) {
         MARS_CUDA_TRY(cudaEventSynchronize(c->used));
         MARS_CUDA_TRY(cudaMemsetAsync(c->d_err, 0, sizeof(int), c->last));
         MARS_CUDA_TRY(cudaEventRecord(c->used, c->last));
+        const int code = *c->h_err;
         *c->h_err = 0;
-        return fail(MARS_ERR_TIMEOUT, "an earlier call's bounded wait gave up: its results are not valid");
+        return fail(MARS_ERR_TIMEOUT, "an earlier call's bounded wait " + std::to_string(code) +
+                                          " gave up: its results are not valid");
     }
     *st = stream != nullptr ? static_cast<cudaStream_t>(stream) : c->stream;
     if (c->any && *st != c->last) {
