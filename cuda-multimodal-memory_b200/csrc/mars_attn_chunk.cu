@@ -51,6 +51,10 @@ constexpr int kThreads = 384;
 constexpr int kUnitCost = 1;                    // a unit's start and end, in tiles
 constexpr float kSlack = 8.0f;                  // how far (log 2) the maximum in use may lag
 constexpr float kLog2e = 1.4426950408889634f;
+// Of 16 pairs of scores, those whose exponential the FMA units take.  The
+// special function unit does 16 a cycle: 2,048 cycles for the two row tiles'
+// 128 keys, all that the products take.  Capped scores need it twice more.
+constexpr int kPolyPlain = 0, kPolyShaped = 0;
 
 template <int kPanels> struct Layout {
     static constexpr int kPanel = kTile * 128;                    // bytes: 128 rows x 64 columns
@@ -87,28 +91,6 @@ __device__ __forceinline__ int key_of(const Unit& u, int t) { return (t < u.n1 ?
 
 // The lowest n bits (n < 0: none, n > 31: all).
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
-
-// Two fp32 values in one register pair.
-__device__ __forceinline__ uint64_t pair(float x, float y) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-    return r;
-}
-__device__ __forceinline__ float2 split(uint64_t v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 
 // ---- shares -----------------------------------------------------------------
 
@@ -421,26 +403,45 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
                     ring.step();
                     vring.step();
                     if (j + 1 < n && !wait(&s_full[ring.slot], ring.phase, 7)) break;
-                    if (j < n0) {
-                        if (!wait(&s_pfull[0], pcount0, 8)) break;
-                        ++pcount0;
-                        tc_fence_after();
-                        outputs(0, vb, j > 0, o_done0);
-                        if (j + 1 < n0) {
-                            if (!after(0, o_done0)) break;
+                    // For each row tile: its weights' product once they are there, then the
+                    // next scores once that is done -- whichever is ready first.
+                    int todo0 = j < n0 ? (j + 1 < n0 ? 2 : 1) : 0, todo1 = j < n1 ? (j + 1 < n1 ? 2 : 1) : 0;
+                    bool out0 = todo0 > 0, out1 = todo1 > 0;      // the product is still to come
+                    uint64_t begin = 0;
+                    for (int look = 1; todo0 + todo1 > 0; ++look) {
+                        if (out0 && warp_try(&s_pfull[0], pcount0 & 1)) {
+                            ++pcount0;
+                            tc_fence_after();
+                            outputs(0, vb, j > 0, o_done0);
+                            out0 = false;
+                            --todo0;
+                        }
+                        if (!out0 && todo0 > 0 && warp_try(&s_odone[0], (o_done0 - 1) & 1)) {
                             scores(0, ring.slot, s_done0);
+                            --todo0;
                         }
-                    }
-                    if (j < n1) {
-                        if (!wait(&s_pfull[1], pcount1, 8)) break;
-                        ++pcount1;
-                        tc_fence_after();
-                        outputs(1, vb, j > 0, o_done1);
-                        if (j + 1 < n1) {
-                            if (!after(1, o_done1)) break;
+                        if (out1 && warp_try(&s_pfull[1], pcount1 & 1)) {
+                            ++pcount1;
+                            tc_fence_after();
+                            outputs(1, vb, j > 0, o_done1);
+                            out1 = false;
+                            --todo1;
+                        }
+                        if (!out1 && todo1 > 0 && warp_try(&s_odone[1], (o_done1 - 1) & 1)) {
                             scores(1, ring.slot, s_done1);
+                            --todo1;
+                        }
+                        if (look % 128 == 0) {        // bounded, as every wait
+                            const uint64_t now = now_ns();
+                            if (begin == 0) begin = now;
+                            if (__any_sync(0xffffffffu, now - begin > kWaitNs || *((volatile int*)w.err) != 0)) {
+                                atomicCAS(w.err, 0, 8);
+                                ok = false;
+                                break;
+                            }
                         }
                     }
+                    if (!ok) break;
                     free_slot();
                     if (j + 1 < n) {
                         free_slot();
@@ -504,6 +505,7 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
         const int t = (warp - 4) >> 2, row = tid - 128 - t * 128;
         const uint32_t tm_s = tmem + ((uint32_t)(warp & 3) << 21) + t * 128;      // lanes of this warp
         const uint32_t tm_o = tm_s + 256;
+        constexpr int kPoly = kShaped ? kPolyShaped : kPolyPlain;
         int scount = 0, ocount = 0;
         for (; more && ok; more = k.next(a, per)) {
             if (t >= k.u.nq) continue;
@@ -526,9 +528,8 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
                 ++scount;
                 tc_fence_after();
                 // the row's 128 scores
-                uint32_t sr[2][64];
-                tmem_load(tm_s, sr[0]);
-                tmem_load(tm_s + 64, sr[1]);
+                uint32_t sr[128];
+                tmem_load(tm_s, sr);
                 const int key0 = key_of(k.u, k.begin + j);
                 const bool all = key0 + kTile <= k.r.prefix || (key0 >= all_lo && key0 + kTile <= all_hi);
                 float f = a.scale * kLog2e, top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -540,17 +541,17 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
                         if (a.cap > 0.0f) {
                             const float in = a.scale / a.cap, out = a.cap * kLog2e;
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) sr[c >> 1][(c & 1) * 32 + i] = __float_as_uint(out * tanh_exp(__uint_as_float(sr[c >> 1][(c & 1) * 32 + i]) * in));
+                            for (int i = 0; i < 32; ++i) sr[c * 32 + i] = __float_as_uint(out * tanh_exp(__uint_as_float(sr[c * 32 + i]) * in));
                         } else {
                             const float g = a.scale * kLog2e;
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) sr[c >> 1][(c & 1) * 32 + i] = __float_as_uint(__uint_as_float(sr[c >> 1][(c & 1) * 32 + i]) * g);
+                            for (int i = 0; i < 32; ++i) sr[c * 32 + i] = __float_as_uint(__uint_as_float(sr[c * 32 + i]) * g);
                         }
                         if (a.decay != nullptr) {
                             const float age = (float)(pos - key0 - c * 32);
 #pragma unroll
                             for (int i = 0; i < 32; ++i)
-                                sr[c >> 1][(c & 1) * 32 + i] = __float_as_uint(fmaf(-decay, fmaxf(age - (float)i, 0.0f), __uint_as_float(sr[c >> 1][(c & 1) * 32 + i])));
+                                sr[c * 32 + i] = __float_as_uint(fmaf(-decay, fmaxf(age - (float)i, 0.0f), __uint_as_float(sr[c * 32 + i])));
                         }
                     }
                     if (!all) {
@@ -558,12 +559,12 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
                         const uint32_t seen = low_bits(pre - kb) | (low_bits(hi - kb) & ~low_bits(lo - kb));
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
-                            if (!((seen >> i) & 1u)) sr[c >> 1][(c & 1) * 32 + i] = 0xff800000u;
+                            if (!((seen >> i) & 1u)) sr[c * 32 + i] = 0xff800000u;
                     }
 #pragma unroll
                     for (int i = 0; i < 32; i += 2)
-                        top4[(i >> 1) & 3] = fmaxf(top4[(i >> 1) & 3],
-                                                   fmaxf(__uint_as_float(sr[c >> 1][(c & 1) * 32 + i]), __uint_as_float(sr[c >> 1][(c & 1) * 32 + i + 1])));
+                        top4[(i >> 1) & 3] = max3(top4[(i >> 1) & 3], __uint_as_float(sr[c * 32 + i]),
+                                                  __uint_as_float(sr[c * 32 + i + 1]));
                 }
                 float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * f;      // f > 0
                 if (__any_sync(0xffffffffu, top > m + kSlack)) {      // m = -inf at first
@@ -590,10 +591,12 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
                     uint32_t p[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float2 e = split(fma2(pair(__uint_as_float(sr[c >> 1][(c & 1) * 32 + 2 * i]), __uint_as_float(sr[c >> 1][(c & 1) * 32 + 2 * i + 1])), f2, base2));
-                        const float x = exp2f_fast(e.x), y = exp2f_fast(e.y);
-                        sum[i & 3] = add2(sum[i & 3], pair(x, y));
-                        p[i] = pack2<T>(x, y);
+                        const float2 e = split(fma2(pair(__uint_as_float(sr[c * 32 + 2 * i]), __uint_as_float(sr[c * 32 + 2 * i + 1])), f2, base2));
+                        float2 y;
+                        if (i % 16 < kPoly) y = exp2_poly(e);
+                        else y = make_float2(exp2f_fast(e.x), exp2f_fast(e.y));
+                        sum[i & 3] = add2(sum[i & 3], pair(y.x, y.y));
+                        p[i] = pack2<T>(y.x, y.y);
                     }
                     tmem_st_32x32b_x16(tm_s + c * 16, p);
                 }
