@@ -4,13 +4,17 @@
 // A unit is 256 rows of one key head (two tiles of 128: tokens x the query
 // heads that share the key head, so one read of keys and values serves them
 // all) against the 128-key tiles that any of its rows sees.  Scores S = Q K^T
-// go to TMEM, a warpgroup for each of the two row tiles turns them into
-// weights P (one thread a row: no shuffles), writes P over S as the second
-// product's operand, and O += P V stays in TMEM for the whole unit:
+// go to TMEM, 64 keys at a time; a warpgroup for each of the two row tiles
+// turns them into weights P (one thread a row: no shuffles), writes P over S as
+// the second product's operand, and O += P V stays in TMEM for the whole unit:
 //
-//    TMEM columns   [0,128) S0/P0   [128,256) S1/P1   [256,384) O0   [384,512) O1
+//    columns  [0,64) S0/P0 first half  [64,128) second half  [128,256) the same
+//             of row tile 1  [256,384) O0  [384,512) O1
 //
-// While one warpgroup exponentiates, the tensor cores work for the other.
+// While a warpgroup works on one half, the other half's weights are multiplied
+// and the next scores are made there, so it never waits for the tensor cores:
+// with scores of 128 keys at once (one buffer) each tile was a chain softmax ->
+// O -> next S of 5,000 cycles for 2,048 cycles of products.
 // The running maximum that P is scaled by follows the true one only when it
 // is 2^8 behind: P stays below 2^8 (harmless in fp32 sums and in the type's
 // relative precision), and O is rescaled a few times a unit instead of at
@@ -18,9 +22,9 @@
 // because the product takes both operands of one type.
 //
 // Roles of a CTA (one on each SM): warp 0 loads by TMA (a lane for each box of
-// a page), warp 1 issues the products, warp 2 zeroes the values of keys that
-// no row sees (they may be anything, and 0 x NaN is NaN), warps 4-7 and 8-11
-// are the two softmax warpgroups.
+// a page), warps 1 and 3 issue the products of row tile 0 and 1, warp 2 zeroes
+// the values of keys that no row sees (they may be anything, and 0 x NaN is
+// NaN), warps 4-7 and 8-11 are the two softmax warpgroups.
 //
 // Work is shared as in mars_attn_short.cu: the units' tiles in one sequence,
 // an equal share for each CTA.  A one-block kernel before it finds the shares
@@ -45,16 +49,13 @@ using namespace mars::sm100;
 
 namespace {
 
-constexpr int kTile = 128;                      // keys
+constexpr int kTile = 128;                      // keys of a ring slot
+constexpr int kHalf = 64;                       // keys of one step of a row tile
 constexpr int kRows = 128;                      // rows of one of the two tiles
 constexpr int kThreads = 384;
 constexpr int kUnitCost = 1;                    // a unit's start and end, in tiles
 constexpr float kSlack = 8.0f;                  // how far (log 2) the maximum in use may lag
 constexpr float kLog2e = 1.4426950408889634f;
-// Of 16 pairs of scores, those whose exponential the FMA units take.  The
-// special function unit does 16 a cycle: 2,048 cycles for the two row tiles'
-// 128 keys, all that the products take.  Capped scores need it twice more.
-constexpr int kPolyPlain = 0, kPolyShaped = 0;
 
 template <int kPanels> struct Layout {
     static constexpr int kPanel = kTile * 128;                    // bytes: 128 rows x 64 columns
@@ -239,7 +240,7 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
     uint8_t* s_q = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* s_kv = s_q + L::kQ;
     __shared__ uint64_t s_qfull, s_qempty, s_full[L::kSlots], s_ready[L::kSlots], s_empty[L::kSlots];
-    __shared__ uint64_t s_sfull[2], s_pfull[2], s_odone[2], s_drain;
+    __shared__ uint64_t s_sfull[2][2], s_pfull[2][2], s_odone[2][2], s_drain[2];      // [row tile][half]
     __shared__ uint32_t s_tmem;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int per = kRows / a.group;              // tokens of a row tile
@@ -247,18 +248,19 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
 
     if (tid == 0) {
         mbar_init(&s_qfull, 1);
-        mbar_init(&s_qempty, 1);
+        mbar_init(&s_qempty, 2);
         for (int i = 0; i < L::kSlots; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&s_ready[i], 1);
-            mbar_init(&s_empty[i], 1);
+            mbar_init(&s_empty[i], 2);
         }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&s_sfull[i], 1);
-            mbar_init(&s_pfull[i], 4);
-            mbar_init(&s_odone[i], 1);
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&s_sfull[i >> 1][i & 1], 1);
+            mbar_init(&s_pfull[i >> 1][i & 1], 4);
+            mbar_init(&s_odone[i >> 1][i & 1], 1);
         }
-        mbar_init(&s_drain, 1);
+        mbar_init(&s_drain[0], 1);
+        mbar_init(&s_drain[1], 1);
         fence_mbar_init();
         prefetch_tmap(&map_q);
         prefetch_tmap(&map_k);
@@ -273,10 +275,8 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
     tc_fence_after();
     const uint32_t tmem = s_tmem;
 
-    // registers: 128 x 88 + 256 x 208 = the 384 x 168 at launch
     bool ok = true;
     if (warp < 4) {
-        set_max_regs<88, false>();
         Walk k;
         bool more = k.start(a, starts, per);
         if (warp == 0) {
@@ -327,121 +327,88 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
             for (int i = max(0, slot_no - L::kSlots); i < slot_no; ++i)
                 drain_wait(&s_full[i % L::kSlots], (i / L::kSlots) & 1, w.err, 3);
             if (q_no > 0) drain_wait(&s_qfull, (q_no - 1) & 1, w.err, 3);
-        } else if (warp == 1) {
-            // ---- products ------------------------------------------------------------
+        } else if (warp != 2) {
+            // ---- products of row tile t ----------------------------------------------
             // The warp stays together: every lane walks and waits, an elected one issues.
             // The operands of tcgen05.mma are uniform registers; in code that a single
             // lane runs by a comparison (lane == 0) they would be copies of that lane's.
+            const int t = warp == 1 ? 0 : 1;
             const uint32_t bf = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
-            const uint32_t idesc_s = idesc_f16(kRows, kTile) | bf;
+            const uint32_t idesc_s = idesc_f16(kRows, kHalf) | bf;
             const uint32_t idesc_o = idesc_f16(kRows, ksteps * 16) | bf | (1u << 16);      // B: columns contiguous
-            // An instruction takes the tensor cores 64 cycles, so what leads up to one has
-            // to be short: of a descriptor only the low word changes, by an add on its
-            // address field (16-byte units).
-            const uint32_t q_lo = (smem_u32(s_q) >> 4) | (1u << 16), kv_lo = (smem_u32(s_kv) >> 4) | (1u << 16);
+            // What leads up to an instruction has to be short: of a descriptor only the low
+            // word changes, by an add on its address field (16-byte units).
+            const uint32_t q_lo = ((smem_u32(s_q) >> 4) | (1u << 16)) + (uint32_t)(t * (kPanels * L::kPanel / 16));
+            const uint32_t k_lo = (smem_u32(s_kv) >> 4) | (1u << 16);
             const uint32_t v_lo = (smem_u32(s_kv) >> 4) | ((uint32_t)L::kPanel >> 4) << 16;
+            const uint32_t tm_s = tmem + t * 128, tm_o = tmem + 256 + t * 128;
             Ring<L::kSlots> ring, vring, freed;       // slots, value tiles, freed slots
-            int pieces = 0, pcount0 = 0, pcount1 = 0;
-            int q_freed = 0, s_done0 = 0, s_done1 = 0, o_done0 = 0, o_done1 = 0;      // commits so far
+            int q_no = 0, steps[2] = {0, 0};          // queries freed; weights multiplied, by half
+            int s_done[2] = {0, 0};                   // scores made, by half
             auto wait = [&](uint64_t* bar, int phase, int code) {
                 ok = ok && warp_wait(bar, phase & 1, w.err, code);
                 return ok;
             };
-            auto scores = [&](int t, int slot, int& done) {      // S_t = Q_t K^T
-                const uint32_t qa = q_lo + (uint32_t)(t * (kPanels * L::kPanel / 16));
-                const uint32_t kb = kv_lo + (uint32_t)(slot * (L::kSlot / 16));
+            // S = Q K^T of 64 keys.  It overwrites P: products with different accumulators
+            // are not ordered by their issue, so the one that reads P has to be done.
+            auto scores = [&](int h, int slot) {
+                if (steps[h] > 0 && !wait(&s_odone[t][h], steps[h] - 1, 13)) return false;
+                tc_fence_after();
+                const uint32_t kb = k_lo + (uint32_t)(slot * (L::kSlot / 16) + h * (kHalf * 128 / 16));
 #pragma unroll
                 for (int ks = 0; ks < 4 * kPanels; ++ks) {
                     const uint32_t off = (uint32_t)((ks >> 2) * (L::kPanel / 16) + (ks & 3) * 2);
                     if (kFull || ks < ksteps) {
-                        if (elect_one()) mma_f16_lo(tmem + t * 128, qa + off, kb + off, idesc_s, ks > 0 ? 1u : 0u);
+                        if (elect_one()) mma_f16_lo(tm_s + h * kHalf, q_lo + off, kb + off, idesc_s, ks > 0 ? 1u : 0u);
                     }
                 }
-                if (elect_one()) mma_commit(&s_sfull[t]);
-                ++done;
+                if (elect_one()) mma_commit(&s_sfull[t][h]);
+                ++s_done[h];
+                return true;
             };
-            auto outputs = [&](int t, uint32_t vb, bool add, int& done) {      // O_t (+)= P_t V
-                // 16 keys a step: 8 columns of P, 2,048 bytes of V
-#pragma unroll
-                for (int ks = 0; ks < kTile / 16; ++ks)
-                    if (elect_one())
-                        mma_f16_ts_lo(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, vb + (uint32_t)(ks * 128), idesc_o,
-                                      add || ks > 0 ? 1u : 0u);
-                if (elect_one()) mma_commit(&s_odone[t]);
-                ++done;
-            };
-            // S_t overwrites P_t.  Products with different accumulators are not ordered
-            // by their issue, so the one that reads P_t has to be done.
-            auto after = [&](int t, int done) { return done == 0 || wait(&s_odone[t], done - 1, 13); };
             auto free_slot = [&] {                    // the ring's next, once the products so far are done
                 if (elect_one()) mma_commit(&s_empty[freed.slot]);
                 freed.step();
             };
             auto free_query = [&] {
                 if (elect_one()) mma_commit(&s_qempty);
-                ++q_freed;
+                ++q_no;
             };
             for (; more && ok; more = k.next(a, per)) {
                 const int n = __shfl_sync(0xffffffffu, k.end - k.begin, 0);
-                const int n0 = __shfl_sync(0xffffffffu, k.count[0], 0), n1 = __shfl_sync(0xffffffffu, k.count[1], 0);
+                const int mine = __shfl_sync(0xffffffffu, t == 0 ? k.count[0] : k.count[1], 0);
                 if (n == 0) continue;
-                if (!wait(&s_qfull, pieces, 4)) break;
+                if (!wait(&s_qfull, q_no, 4)) break;
                 if (!wait(&s_full[ring.slot], ring.phase, 5)) break;
-                if (n0 > 0 && !after(0, o_done0)) break;
-                if (n1 > 0 && !after(1, o_done1)) break;
-                tc_fence_after();
-                if (n0 > 0) scores(0, ring.slot, s_done0);
-                if (n1 > 0) scores(1, ring.slot, s_done1);
+                if (mine > 0 && !(scores(0, ring.slot) && scores(1, ring.slot))) break;
                 free_slot();
                 if (n == 1) free_query();
                 ring.step();
                 for (int j = 0; j < n && ok; ++j) {
                     // here: values of tile j; then keys of tile j + 1
                     if (!wait(&s_full[ring.slot], ring.phase, 6)) break;
-                    if (!wait(&s_ready[vring.slot], vring.phase, 6)) break;
+                    if (!wait(&s_ready[vring.slot], vring.phase, 7)) break;
                     const uint32_t vb = v_lo + (uint32_t)(ring.slot * (L::kSlot / 16));
                     ring.step();
                     vring.step();
-                    if (j + 1 < n && !wait(&s_full[ring.slot], ring.phase, 7)) break;
-                    // For each row tile: its weights' product once they are there, then the
-                    // next scores once that is done -- whichever is ready first.
-                    int todo0 = j < n0 ? (j + 1 < n0 ? 2 : 1) : 0, todo1 = j < n1 ? (j + 1 < n1 ? 2 : 1) : 0;
-                    bool out0 = todo0 > 0, out1 = todo1 > 0;      // the product is still to come
-                    uint64_t begin = 0;
-                    for (int look = 1; todo0 + todo1 > 0; ++look) {
-                        if (out0 && warp_try(&s_pfull[0], pcount0 & 1)) {
-                            ++pcount0;
+                    if (j + 1 < n && !wait(&s_full[ring.slot], ring.phase, 8)) break;
+                    if (j < mine) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if (!wait(&s_pfull[t][h], steps[h], 9)) break;
                             tc_fence_after();
-                            outputs(0, vb, j > 0, o_done0);
-                            out0 = false;
-                            --todo0;
+                            // O (+)= P V: 16 keys a step, 8 columns of P, 2,048 bytes of V
+#pragma unroll
+                            for (int ks = 0; ks < kHalf / 16; ++ks)
+                                if (elect_one())
+                                    mma_f16_ts_lo(tm_o, tm_s + h * kHalf + ks * 8, vb + (uint32_t)((h * 4 + ks) * 128), idesc_o,
+                                                  j > 0 || h > 0 || ks > 0 ? 1u : 0u);
+                            if (elect_one()) mma_commit(&s_odone[t][h]);
+                            ++steps[h];
+                            if (j + 1 < mine && !scores(h, ring.slot)) break;
                         }
-                        if (!out0 && todo0 > 0 && warp_try(&s_odone[0], (o_done0 - 1) & 1)) {
-                            scores(0, ring.slot, s_done0);
-                            --todo0;
-                        }
-                        if (out1 && warp_try(&s_pfull[1], pcount1 & 1)) {
-                            ++pcount1;
-                            tc_fence_after();
-                            outputs(1, vb, j > 0, o_done1);
-                            out1 = false;
-                            --todo1;
-                        }
-                        if (!out1 && todo1 > 0 && warp_try(&s_odone[1], (o_done1 - 1) & 1)) {
-                            scores(1, ring.slot, s_done1);
-                            --todo1;
-                        }
-                        if (look % 128 == 0) {        // bounded, as every wait
-                            const uint64_t now = now_ns();
-                            if (begin == 0) begin = now;
-                            if (__any_sync(0xffffffffu, now - begin > kWaitNs || *((volatile int*)w.err) != 0)) {
-                                atomicCAS(w.err, 0, 8);
-                                ok = false;
-                                break;
-                            }
-                        }
+                        if (!ok) break;
                     }
-                    if (!ok) break;
                     free_slot();
                     if (j + 1 < n) {
                         free_slot();
@@ -449,24 +416,25 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
                     }
                     if (j + 2 == n) free_query();
                 }
-                ++pieces;
             }
             // No product may be in flight when TMEM is freed, and no commit's arrival
-            // when the CTA's shared memory is: the last of each barrier is awaited,
-            // those that no role waits for among them.
-            if (elect_one()) mma_commit(&s_drain);
-            drain_wait(&s_drain, 0, w.err, 9);
-            for (int i = 0; i < L::kSlots; ++i) {     // slot i's last use: this round's, or the one before
-                const int uses = freed.rounds + (i < freed.slot);
-                if (uses > 0) drain_wait(&s_empty[i], (uses - 1) & 1, w.err, 9);
+            // when the CTA's shared memory is: the last of each barrier is awaited, those
+            // that no role waits for among them.
+            if (elect_one()) mma_commit(&s_drain[t]);
+            drain_wait(&s_drain[t], 0, w.err, 9);
+            if (ok) {                                 // both row tiles' arrivals
+                for (int i = 0; i < L::kSlots; ++i) { // slot i's last use: this round's, or the one before
+                    const int uses = freed.rounds + (i < freed.slot);
+                    if (uses > 0) drain_wait(&s_empty[i], (uses - 1) & 1, w.err, 9);
+                }
+                if (q_no > 0) drain_wait(&s_qempty, (q_no - 1) & 1, w.err, 9);
             }
-            if (q_freed > 0) drain_wait(&s_qempty, (q_freed - 1) & 1, w.err, 9);
-            if (s_done0 > 0) drain_wait(&s_sfull[0], (s_done0 - 1) & 1, w.err, 9);
-            if (s_done1 > 0) drain_wait(&s_sfull[1], (s_done1 - 1) & 1, w.err, 9);
-            if (o_done0 > 0) drain_wait(&s_odone[0], (o_done0 - 1) & 1, w.err, 9);
-            if (o_done1 > 0) drain_wait(&s_odone[1], (o_done1 - 1) & 1, w.err, 9);
+            for (int h = 0; h < 2; ++h) {
+                if (s_done[h] > 0) drain_wait(&s_sfull[t][h], (s_done[h] - 1) & 1, w.err, 9);
+                if (steps[h] > 0) drain_wait(&s_odone[t][h], (steps[h] - 1) & 1, w.err, 9);
+            }
             __syncwarp();
-        } else if (warp == 2) {
+        } else {
             // ---- values that no row sees ----------------------------------------------
             Ring<L::kSlots> ring, vring;
             for (; more && ok; more = k.next(a, per)) {
@@ -499,17 +467,15 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
         }
     } else {
         // ---- softmax: warpgroup t, a thread for each row ------------------------------
-        set_max_regs<208, true>();
         Walk k;
         bool more = k.start(a, starts, per);
         const int t = (warp - 4) >> 2, row = tid - 128 - t * 128;
         const uint32_t tm_s = tmem + ((uint32_t)(warp & 3) << 21) + t * 128;      // lanes of this warp
         const uint32_t tm_o = tm_s + 256;
-        constexpr int kPoly = kShaped ? kPolyShaped : kPolyPlain;
-        int scount = 0, ocount = 0;
+        int seen_tiles = 0;                       // the phase of each half's barriers
         for (; more && ok; more = k.next(a, per)) {
             if (t >= k.u.nq) continue;
-            const int n = k.count[t];
+            const int n = t == 0 ? k.count[0] : k.count[1];
             const int tok0 = k.u.row0 + t * per, toks = min(per, k.u.rows - t * per);
             const int tok = tok0 + row / a.group, head = k.cur.h * a.group + row % a.group;
             const bool valid = row < toks * a.group;
@@ -522,100 +488,100 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
             const int all_hi = min(k.r.len, first_pos + 1), all_lo = a.window > 0 ? first_pos + toks - a.window : 0;
             float m = -INFINITY, l = 0.0f;
 
-            for (int j = 0; j < n; ++j) {
-                ok = ok && warp_wait(&s_sfull[t], scount & 1, w.err, 11);
-                if (!ok) break;
-                ++scount;
-                tc_fence_after();
-                // the row's 128 scores
-                uint32_t sr[128];
-                tmem_load(tm_s, sr);
-                const int key0 = key_of(k.u, k.begin + j);
-                const bool all = key0 + kTile <= k.r.prefix || (key0 >= all_lo && key0 + kTile <= all_hi);
-                float f = a.scale * kLog2e, top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                if (kShaped) f = 1.0f;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
+            for (int j = 0; j < n && ok; ++j) {
+                const int key_tile = key_of(k.u, k.begin + j);
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
+                    ok = ok && warp_wait(&s_sfull[t][h], seen_tiles & 1, w.err, 11);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t tm = tm_s + h * kHalf;
+                    uint32_t sr[kHalf];               // the row's scores
+                    tmem_load(tm, sr);
+                    const int key0 = key_tile + h * kHalf;
+                    const bool all = key0 + kHalf <= k.r.prefix || (key0 >= all_lo && key0 + kHalf <= all_hi);
+                    float f = a.scale * kLog2e, top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                     if (kShaped) {
                         // the score in units of log 2 itself
                         if (a.cap > 0.0f) {
                             const float in = a.scale / a.cap, out = a.cap * kLog2e;
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) sr[c * 32 + i] = __float_as_uint(out * tanh_exp(__uint_as_float(sr[c * 32 + i]) * in));
+                            for (int i = 0; i < kHalf; ++i)
+                                sr[i] = __float_as_uint(out * tanh_exp(__uint_as_float(sr[i]) * in));
                         } else {
-                            const float g = a.scale * kLog2e;
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) sr[c * 32 + i] = __float_as_uint(__uint_as_float(sr[c * 32 + i]) * g);
+                            for (int i = 0; i < kHalf; ++i) sr[i] = __float_as_uint(__uint_as_float(sr[i]) * f);
                         }
                         if (a.decay != nullptr) {
-                            const float age = (float)(pos - key0 - c * 32);
+                            const float age = (float)(pos - key0);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                sr[c * 32 + i] = __float_as_uint(fmaf(-decay, fmaxf(age - (float)i, 0.0f), __uint_as_float(sr[c * 32 + i])));
+                            for (int i = 0; i < kHalf; ++i)
+                                sr[i] = __float_as_uint(fmaf(-decay, fmaxf(age - (float)i, 0.0f), __uint_as_float(sr[i])));
                         }
+                        f = 1.0f;
                     }
                     if (!all) {
-                        const int kb = key0 + c * 32;
-                        const uint32_t seen = low_bits(pre - kb) | (low_bits(hi - kb) & ~low_bits(lo - kb));
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (!((seen >> i) & 1u)) sr[c * 32 + i] = 0xff800000u;
-                    }
+                        for (int c = 0; c < 2; ++c) {
+                            const int kb = key0 + c * 32;
+                            const uint32_t seen = low_bits(pre - kb) | (low_bits(hi - kb) & ~low_bits(lo - kb));
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2)
-                        top4[(i >> 1) & 3] = max3(top4[(i >> 1) & 3], __uint_as_float(sr[c * 32 + i]),
-                                                  __uint_as_float(sr[c * 32 + i + 1]));
-                }
-                float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * f;      // f > 0
-                if (__any_sync(0xffffffffu, top > m + kSlack)) {      // m = -inf at first
-                    const float to = fmaxf(top, m);
-                    const float keep = to == -INFINITY ? 1.0f : exp2f_fast(m - to);
-                    if (j > 0) {
-                        // O of the tiles before: complete, since S of this one was issued after them
-                        for (int c = 0; c * 32 < a.D; ++c) {
-                            uint32_t o[32];
-                            tmem_load(tm_o + c * 32, o);
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
-                            tmem_st_32x32b_x32(tm_o + c * 32, o);
+                            for (int i = 0; i < 32; ++i)
+                                if (!((seen >> i) & 1u)) sr[c * 32 + i] = 0xff800000u;
                         }
                     }
-                    l *= keep;
-                    m = to;
-                }
-                const float base = m == -INFINITY ? 0.0f : m;
-                const uint64_t f2 = pair(f, f), base2 = pair(-base, -base);
-                uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t p[16];
+                    for (int i = 0; i < kHalf; i += 2)
+                        top4[(i >> 1) & 3] = max3(top4[(i >> 1) & 3], __uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
+                    const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * f;      // f > 0
+                    if (__any_sync(0xffffffffu, top > m + kSlack)) {      // m = -inf at first
+                        const float to = fmaxf(top, m);
+                        const float keep = to == -INFINITY ? 1.0f : exp2f_fast(m - to);
+                        if (j + h > 0) {
+                            // once the products of the steps before are in O
+                            ok = ok && warp_wait(&s_odone[t][h ^ 1], (seen_tiles + h + 1) & 1, w.err, 14);
+                            if (!ok) break;
+                            tc_fence_after();
+                            for (int c = 0; c * 32 < a.D; ++c) {
+                                uint32_t o[32];
+                                tmem_load(tm_o + c * 32, o);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float2 e = split(fma2(pair(__uint_as_float(sr[c * 32 + 2 * i]), __uint_as_float(sr[c * 32 + 2 * i + 1])), f2, base2));
-                        float2 y;
-                        if (i % 16 < kPoly) y = exp2_poly(e);
-                        else y = make_float2(exp2f_fast(e.x), exp2f_fast(e.y));
-                        sum[i & 3] = add2(sum[i & 3], pair(y.x, y.y));
-                        p[i] = pack2<T>(y.x, y.y);
+                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+                                tmem_st_32x32b_x32(tm_o + c * 32, o);
+                            }
+                        }
+                        l *= keep;
+                        m = to;
                     }
-                    tmem_st_32x32b_x16(tm_s + c * 16, p);
+                    const float base = m == -INFINITY ? 0.0f : m;
+                    const uint64_t f2 = pair(f, f), base2 = pair(-base, -base);
+                    uint64_t sum[4] = {0, 0, 0, 0};
+                    uint32_t p[kHalf / 2];
+#pragma unroll
+                    for (int i = 0; i < kHalf / 2; ++i) {
+                        const float2 e = split(fma2(pair(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), f2, base2));
+                        const float x = exp2f_fast(e.x), y = exp2f_fast(e.y);
+                        sum[i & 3] = add2(sum[i & 3], pair(x, y));
+                        p[i] = pack2<T>(x, y);
+                    }
+                    tmem_st_32x32b_x32(tm, p);
+                    {
+                        const float2 e = split(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
+                        l += e.x + e.y;
+                    }
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s_pfull[t][h]);
                 }
-                {
-                    const float2 e = split(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
-                    l += e.x + e.y;
-                }
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&s_pfull[t]);
+                ++seen_tiles;
             }
             if (!ok) break;
 
             // ---- the piece's end -------------------------------------------------
-            // the product of the last tile (those before it were done when its scores came)
+            // the product of the last step, which those before it are part of
             if (n > 0) {
-                ocount += n;
-                ok = ok && warp_wait(&s_odone[t], (ocount - 1) & 1, w.err, 12);
+                ok = ok && warp_wait(&s_odone[t][1], (seen_tiles - 1) & 1, w.err, 12);
                 if (!ok) break;
                 tc_fence_after();
             }

@@ -72,10 +72,6 @@ __device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, int
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
     return __all_sync(0xffffffffu, bounded_wait(bar, parity, err, code, false));
 }
-// One look at a barrier, for all lanes of a warp.
-__device__ __forceinline__ bool warp_try(uint64_t* bar, uint32_t parity) {
-    return __all_sync(0xffffffffu, sm100::mbar_try_wait(bar, parity));
-}
 __device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
     bounded_wait(bar, parity, err, code, true);
 }
@@ -149,27 +145,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-// 2^x of two values below 2^7 by the FMA units, beside the special function
-// unit's 16 a cycle: x = n + r with n the nearest whole number (adding 1.5 x
-// 2^23 leaves it in the low bits), 2^r by a polynomial of degree 5 fitted here
-// to the least largest relative error on [-1/2, 1/2] (2^-22.5 in fp32), and n
-// added to the exponent.  From -127 down the result is 0.
-__device__ __forceinline__ float2 exp2_poly(float2 v) {
-    const uint64_t magic = pair(12582912.0f, 12582912.0f), back = pair(-12582912.0f, -12582912.0f);
-    const uint64_t x = pair(fmaxf(v.x, -127.0f), fmaxf(v.y, -127.0f));
-    const uint64_t t = add2(x, magic);
-    const uint64_t r = fma2(add2(t, back), pair(-1.0f, -1.0f), x);
-    uint64_t p = pair(0.001326472731307149f, 0.001326472731307149f);
-    p = fma2(p, r, pair(0.009671512991189957f, 0.009671512991189957f));
-    p = fma2(p, r, pair(0.05550733581185341f, 0.05550733581185341f));
-    p = fma2(p, r, pair(0.24022242426872253f, 0.24022242426872253f));
-    p = fma2(p, r, pair(0.6931470036506653f, 0.6931470036506653f));
-    p = fma2(p, r, pair(1.0f, 1.0f));
-    const float2 n = split(t), q = split(p);
-    return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(n.x) << 23)),
-                       __int_as_float(__float_as_int(q.y) + (__float_as_int(n.y) << 23)));
-}
-
 // Two values rounded to T, the first in the low half.
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
@@ -233,17 +208,13 @@ __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) {
           "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr) : "memory");
 }
-__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[128]) {
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[64]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
         "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
         "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
         "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
-        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,"
-        "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
-        "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
-        "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
-        "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%128];\n\t"
+        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
         "tcgen05.wait::ld.sync.aligned;"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
@@ -252,15 +223,7 @@ __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[128]) {
           "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
           "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
           "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
-          "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
-          "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
-          "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
-          "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
-          "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
-          "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]),
-          "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
-          "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
         : "r"(taddr) : "memory");
 }
 
@@ -275,21 +238,7 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
           "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
-        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
-        : "memory");
-}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-// Registers of the calling warpgroup from here on.
-template <int kRegs, bool kMore> __device__ __forceinline__ void set_max_regs() {
-    if (kMore) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
-    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
-}
 
 // Host side (mars_attn.cu).
 // The largest power of two that divides a page and a tile of keys.
