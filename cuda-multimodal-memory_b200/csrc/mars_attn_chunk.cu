@@ -355,14 +355,15 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
                 if (steps[h] > 0 && !wait(&s_odone[t][h], steps[h] - 1, 13)) return false;
                 tc_fence_after();
                 const uint32_t kb = k_lo + (uint32_t)(slot * (L::kSlot / 16) + h * (kHalf * 128 / 16));
-#pragma unroll
-                for (int ks = 0; ks < 4 * kPanels; ++ks) {
-                    const uint32_t off = (uint32_t)((ks >> 2) * (L::kPanel / 16) + (ks & 3) * 2);
-                    if (kFull || ks < ksteps) {
+                if (kFull) {
+                    mma_scores<kPanels>(tm_s + h * kHalf, q_lo, kb, idesc_s, &s_sfull[t][h]);
+                } else {
+                    for (int ks = 0; ks < ksteps; ++ks) {
+                        const uint32_t off = (uint32_t)((ks >> 2) * (L::kPanel / 16) + (ks & 3) * 2);
                         if (elect_one()) mma_f16_lo(tm_s + h * kHalf, q_lo + off, kb + off, idesc_s, ks > 0 ? 1u : 0u);
                     }
+                    if (elect_one()) mma_commit(&s_sfull[t][h]);
                 }
-                if (elect_one()) mma_commit(&s_sfull[t][h]);
                 ++s_done[h];
                 return true;
             };
@@ -397,13 +398,9 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
                         for (int h = 0; h < 2; ++h) {
                             if (!wait(&s_pfull[t][h], steps[h], 9)) break;
                             tc_fence_after();
-                            // O (+)= P V: 16 keys a step, 8 columns of P, 2,048 bytes of V
-#pragma unroll
-                            for (int ks = 0; ks < kHalf / 16; ++ks)
-                                if (elect_one())
-                                    mma_f16_ts_lo(tm_o, tm_s + h * kHalf + ks * 8, vb + (uint32_t)((h * 4 + ks) * 128), idesc_o,
-                                                  j > 0 || h > 0 || ks > 0 ? 1u : 0u);
-                            if (elect_one()) mma_commit(&s_odone[t][h]);
+                            // O (+)= P V
+                            mma_weights(tm_o, tm_s + h * kHalf, vb + (uint32_t)(h * (kHalf * 128 / 16)), idesc_o, j + h > 0,
+                                        &s_odone[t][h]);
                             ++steps[h];
                             if (j + 1 < mine && !scores(h, ring.slot)) break;
                         }

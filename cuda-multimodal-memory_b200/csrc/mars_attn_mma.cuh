@@ -180,16 +180,72 @@ __device__ __forceinline__ void mma_f16_lo(uint32_t tmem_d, uint32_t a_lo, uint3
                  : "memory");
 }
 
-// D[tmem] (+)= A[tmem] x B[smem], kind::f16: A's rows are lanes, two values a
-// column; B's N index is contiguous, rows of 64 values are consecutive K.
-__device__ __forceinline__ void mma_f16_ts_lo(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t idesc,
-                                              uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
-                 "setp.ne.b32 p, %4, 0;\n\t"
-                 "mov.b64 db, {%2, %5};\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}"
-                 ::"r"(tmem_d), "r"(tmem_a), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
-                 : "memory");
+// A step's products by one elected lane of a converged warp, and the commit of
+// what the lane issued so far to `bar`.  One statement, predicated by
+// elect.sync: a branch around each instruction cost 110 cycles an instruction
+// where the tensor cores take 48 to 64.
+// D[tmem] = A[smem] x B[smem]^T over 64 kPanels columns (kPanel bytes between
+// the blocks of 64).
+template <int kPanels>
+__device__ __forceinline__ void mma_scores(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint64_t* bar) {
+    if (kPanels == 1)
+        asm volatile(
+        "{\n\t.reg .pred e, p, q;\n\t.reg .b64 a, b;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, 0, 0;\n\tsetp.eq.b32 q, 0, 0;\n\t"
+        "mov.b64 a, {%1, %4};\n\tmov.b64 b, {%2, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t"
+        "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, q;\n\t"
+        "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, q;\n\t"
+        "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, q;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t}"
+        ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(idesc), "n"(kDescHigh), "r"(sm100::smem_u32(bar)) : "memory");
+    else
+        asm volatile(
+        "{\n\t.reg .pred e, p, q;\n\t.reg .b64 a, b;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, 0, 0;\n\tsetp.eq.b32 q, 0, 0;\n\t"
+        "mov.b64 a, {%1, %4};\n\tmov.b64 b, {%2, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t"
+        "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, q;\n\t"
+        "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, q;\n\t"
+        "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, q;\n\t"
+        "add.s64 a, a, 1018;\n\tadd.s64 b, b, 1018;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, q;\n\t"
+        "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, q;\n\t"
+        "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, q;\n\t"
+        "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, q;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t}"
+        ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(idesc), "n"(kDescHigh), "r"(sm100::smem_u32(bar)) : "memory");
+}
+// D[tmem] (+)= A[tmem] x B[smem] over 64 rows of B (8 columns of A and 2,048
+// bytes of B an instruction).
+__device__ __forceinline__ void mma_weights(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t idesc, bool add,
+                                            uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred e, p, q;\n\t.reg .b64 b;\n\t.reg .b32 a;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 q, 0, 0;\n\t"
+        "mov.b32 a, %1;\n\tmov.b64 b, {%2, %5};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, p;\n\t"
+        "add.s32 a, a, 8;\n\tadd.s64 b, b, 128;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, q;\n\t"
+        "add.s32 a, a, 8;\n\tadd.s64 b, b, 128;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, q;\n\t"
+        "add.s32 a, a, 8;\n\tadd.s64 b, b, 128;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, q;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%6];\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "r"(b_lo), "r"(idesc), "r"((uint32_t)add), "n"(kDescHigh), "r"(sm100::smem_u32(bar))
+        : "memory");
 }
 
 // 32 lanes x N consecutive columns, complete on return: load and wait are one
