@@ -342,9 +342,10 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
             const uint32_t k_lo = (smem_u32(s_kv) >> 4) | (1u << 16);
             const uint32_t v_lo = (smem_u32(s_kv) >> 4) | ((uint32_t)L::kPanel >> 4) << 16;
             const uint32_t tm_s = tmem + t * 128, tm_o = tmem + 256 + t * 128;
-            Ring<L::kSlots> ring, vring, freed;       // slots, value tiles, freed slots
+            Ring<L::kSlots> keys, vals, vready;       // the ring's slots of keys and values (every other one), value tiles
+            vals.step();
             int q_no = 0, steps[2] = {0, 0};          // queries freed; weights multiplied, by half
-            int s_done[2] = {0, 0};                   // scores made, by half
+            int s_done = 0;                           // scores made of second halves
             auto wait = [&](uint64_t* bar, int phase, int code) {
                 ok = ok && warp_wait(bar, phase & 1, w.err, code);
                 return ok;
@@ -352,7 +353,6 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
             // S = Q K^T of 64 keys.  It overwrites P: products with different accumulators
             // are not ordered by their issue, so the one that reads P has to be done.
             auto scores = [&](int h, int slot) {
-                if (steps[h] > 0 && !wait(&s_odone[t][h], steps[h] - 1, 13)) return false;
                 tc_fence_after();
                 const uint32_t kb = k_lo + (uint32_t)(slot * (L::kSlot / 16) + h * (kHalf * 128 / 16));
                 if (kFull) {
@@ -364,72 +364,83 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
                     }
                     if (elect_one()) mma_commit(&s_sfull[t][h]);
                 }
-                ++s_done[h];
+                s_done += h;
+            };
+            // O (+)= P V of 64 keys, once the weights are there.
+            auto outputs = [&](int h, bool add) {
+                if (!wait(&s_pfull[t][h], steps[h], 9)) return false;
+                tc_fence_after();
+                mma_weights(tm_o, tm_s + h * kHalf, v_lo + (uint32_t)(vals.slot * (L::kSlot / 16) + h * (kHalf * 128 / 16)), idesc_o,
+                            add, &s_odone[t][h]);
+                ++steps[h];
                 return true;
             };
-            auto free_slot = [&] {                    // the ring's next, once the products so far are done
-                if (elect_one()) mma_commit(&s_empty[freed.slot]);
-                freed.step();
-            };
-            auto free_query = [&] {
-                if (elect_one()) mma_commit(&s_qempty);
-                ++q_no;
+            auto outputs_done = [&](int h) { return steps[h] == 0 || wait(&s_odone[t][h], steps[h] - 1, 13); };
+            auto values_there = [&] { return wait(&s_full[vals.slot], vals.phase, 6) && wait(&s_ready[vready.slot], vready.phase, 7); };
+            auto two_on = [](Ring<L::kSlots>& r) { r.step(); r.step(); };
+            // What frees a slot is known here without a commit of its own (which would wait
+            // in the queue behind the products): weights follow from finished scores, and
+            // S waits for finished outputs.
+            auto free = [&](uint64_t* bar) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar);
             };
             for (; more && ok; more = k.next(a, per)) {
                 const int n = __shfl_sync(0xffffffffu, k.end - k.begin, 0);
                 const int mine = __shfl_sync(0xffffffffu, t == 0 ? k.count[0] : k.count[1], 0);
                 if (n == 0) continue;
-                if (!wait(&s_qfull, q_no, 4)) break;
-                if (!wait(&s_full[ring.slot], ring.phase, 5)) break;
-                if (mine > 0 && !(scores(0, ring.slot) && scores(1, ring.slot))) break;
-                free_slot();
-                if (n == 1) free_query();
-                ring.step();
-                for (int j = 0; j < n && ok; ++j) {
-                    // here: values of tile j; then keys of tile j + 1
-                    if (!wait(&s_full[ring.slot], ring.phase, 6)) break;
-                    if (!wait(&s_ready[vring.slot], vring.phase, 7)) break;
-                    const uint32_t vb = v_lo + (uint32_t)(ring.slot * (L::kSlot / 16));
-                    ring.step();
-                    vring.step();
-                    if (j + 1 < n && !wait(&s_full[ring.slot], ring.phase, 8)) break;
-                    if (j < mine) {
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            if (!wait(&s_pfull[t][h], steps[h], 9)) break;
-                            tc_fence_after();
-                            // O (+)= P V
-                            mma_weights(tm_o, tm_s + h * kHalf, vb + (uint32_t)(h * (kHalf * 128 / 16)), idesc_o, j + h > 0,
-                                        &s_odone[t][h]);
-                            ++steps[h];
-                            if (j + 1 < mine && !scores(h, ring.slot)) break;
-                        }
-                        if (!ok) break;
-                    }
-                    free_slot();
-                    if (j + 1 < n) {
-                        free_slot();
-                        ring.step();
-                    }
-                    if (j + 2 == n) free_query();
+                if (!wait(&s_qfull, q_no, 4) || !wait(&s_full[keys.slot], keys.phase, 5)) break;
+                if (mine > 0) {
+                    if (!outputs_done(0) || !outputs_done(1)) break;
+                    scores(0, keys.slot);
+                    scores(1, keys.slot);
+                    if (!values_there()) break;
                 }
+#pragma unroll 1
+                for (int j = 0; j < mine && ok; ++j) {
+                    // here: scores of tile j made, its values there.  The waits for what comes by
+                    // TMA stand where the products' own take time.
+                    const bool next = j + 1 < mine;
+                    uint64_t* this_keys = &s_empty[keys.slot];
+                    uint64_t* this_vals = &s_empty[vals.slot];
+                    two_on(keys);
+                    if (!outputs(0, j > 0)) break;
+                    if (j + 1 < n && !wait(&s_full[keys.slot], keys.phase, 8)) break;
+                    if (next) {
+                        if (!outputs_done(0)) break;
+                        scores(0, keys.slot);
+                    }
+                    if (!outputs(1, true)) break;
+                    free(this_keys);
+                    if (j + 1 == n) free(&s_qempty);
+                    two_on(vals);
+                    vready.step();
+                    if (next && !values_there()) break;
+                    if (!outputs_done(1)) break;
+                    free(this_vals);
+                    if (next) scores(1, keys.slot);
+                }
+                if (!ok) break;
+                // tiles that only the other row tile sees
+#pragma unroll 1
+                for (int j = mine; j < n; ++j) {
+                    if (!wait(&s_full[keys.slot], keys.phase, 5) || !values_there()) break;
+                    free(&s_empty[keys.slot]);
+                    free(&s_empty[vals.slot]);
+                    if (j + 1 == n) free(&s_qempty);
+                    two_on(keys);
+                    two_on(vals);
+                    vready.step();
+                }
+                ++q_no;
             }
             // No product may be in flight when TMEM is freed, and no commit's arrival
-            // when the CTA's shared memory is: the last of each barrier is awaited, those
-            // that no role waits for among them.
+            // when the CTA's shared memory is: the last of each barrier is awaited.
             if (elect_one()) mma_commit(&s_drain[t]);
-            drain_wait(&s_drain[t], 0, w.err, 9);
-            if (ok) {                                 // both row tiles' arrivals
-                for (int i = 0; i < L::kSlots; ++i) { // slot i's last use: this round's, or the one before
-                    const int uses = freed.rounds + (i < freed.slot);
-                    if (uses > 0) drain_wait(&s_empty[i], (uses - 1) & 1, w.err, 9);
-                }
-                if (q_no > 0) drain_wait(&s_qempty, (q_no - 1) & 1, w.err, 9);
-            }
-            for (int h = 0; h < 2; ++h) {
-                if (s_done[h] > 0) drain_wait(&s_sfull[t][h], (s_done[h] - 1) & 1, w.err, 9);
-                if (steps[h] > 0) drain_wait(&s_odone[t][h], (steps[h] - 1) & 1, w.err, 9);
-            }
+            drain_wait(&s_drain[t], 0, w.err, 10);
+            if (steps[0] > 0) drain_wait(&s_odone[t][0], (steps[0] - 1) & 1, w.err, 10);
+            if (steps[1] > 0) drain_wait(&s_odone[t][1], (steps[1] - 1) & 1, w.err, 10);
+            if (s_done > 0) drain_wait(&s_sfull[t][1], (s_done - 1) & 1, w.err, 10);
             __syncwarp();
         } else {
             // ---- values that no row sees ----------------------------------------------

@@ -60,11 +60,17 @@ __device__ __forceinline__ uint64_t now_ns() {
 }
 __device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, int* err, int code, bool drain) {
     if (sm100::mbar_try_wait(bar, parity)) return true;
-    const uint64_t begin = now_ns();
-    for (;;) {
-        for (int i = 0; i < 64; ++i)
-            if (sm100::mbar_try_wait(bar, parity)) return true;
-        if (now_ns() - begin > kWaitNs || (!drain && *((volatile int*)err) != 0)) break;
+    // Kept small (unrolled, the polls of twenty waits were most of a 148 KB
+    // kernel, and its path through them missed the instruction cache).
+    uint64_t begin = 0;
+#pragma unroll 1
+    for (uint32_t i = 1;; ++i) {
+        if (sm100::mbar_try_wait(bar, parity)) return true;
+        if ((i & 63u) == 0) {
+            const uint64_t now = now_ns();
+            if (begin == 0) begin = now;
+            if (now - begin > kWaitNs || (!drain && *((volatile int*)err) != 0)) break;
+        }
     }
     atomicCAS(err, 0, code);
     return false;
