@@ -733,5 +733,6 @@ _KV_NAMES = ("KvCache", "KvContext", "KvPlan", "rope", "rope_append", "KV_MAX_RE
 def __getattr__(name):
     if name in _KV_NAMES:
         from . import kv
-        return getattr(kv, name)
+        globals().update({n: getattr(kv, n) for n in _KV_NAMES})
+        return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -21,7 +21,10 @@ from typing import NamedTuple
 
 import torch
 
-from . import _check, _stream, lib
+from . import _STREAM_LEGACY, _check, lib
+
+_raw_stream = torch._C._cuda_getCurrentRawStream      # torch.cuda.current_stream(...).cuda_stream without its objects
+_current_device = torch._C._cuda_getDevice
 
 KV_MAX_REQUESTS = 8192   # MARS_KV_MAX_REQUESTS
 
@@ -43,12 +46,29 @@ class KvPlan(NamedTuple):
     status: torch.Tensor       # [1] 0, or KV_* bits: then nothing was handed out
 
 
+def _stream(stream, t):
+    """The given stream, or torch's current one on t's device (as the other calls of this package do)."""
+    if stream is not None:
+        return stream
+    return _raw_stream(t.get_device()) or _STREAM_LEGACY
+
+
+def _on_device_of(t, call, args):
+    """call(*args) with t's device as the current one, for entry points without a context."""
+    if t.get_device() == _current_device():
+        _check(call(*args))
+    else:
+        with torch.cuda.device(t.device):
+            _check(call(*args))
+
+
 def _ints(name, t, n=None, dims=1):
     """The address of a contiguous int32 CUDA tensor of n entries (n None: any)."""
-    if t.dtype is not torch.int32 or not t.is_cuda or not t.is_contiguous() or t.dim() != dims:
+    shape = t.shape
+    if t.dtype is not torch.int32 or not t.is_cuda or len(shape) != dims or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 CUDA tensor of {dims} dimension(s)")
-    if n is not None and t.shape[0] != n:
-        raise ValueError(f"{name} must have {n} entries, has {t.shape[0]}")
+    if n is not None and shape[0] != n:
+        raise ValueError(f"{name} must have {n} entries, has {shape[0]}")
     return t.data_ptr()
 
 
@@ -59,7 +79,8 @@ class _Cache(C.Structure):
     """mars_kv_cache."""
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int32), ("num_pages", C.c_int32),
                 ("page_size", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("reserved", C.c_int32),
-                ("k_strides", C.c_int64 * 3), ("v_strides", C.c_int64 * 3)]
+                ("k_page_stride", C.c_int64), ("k_slot_stride", C.c_int64), ("k_head_stride", C.c_int64),
+                ("v_page_stride", C.c_int64), ("v_slot_stride", C.c_int64), ("v_head_stride", C.c_int64)]
 
 
 class _Table(C.Structure):
@@ -78,26 +99,27 @@ class KvCache:
     strides with contiguous columns -- a permuted view where memory has the heads before the tokens."""
 
     def __init__(self, k, v):
-        if k.shape != v.shape or k.dtype is not v.dtype or k.dim() != 4 or k.device != v.device or not k.is_cuda:
+        shape, dtype = k.shape, k.dtype
+        if v.shape != shape or v.dtype is not dtype or len(shape) != 4 or not k.is_cuda or k.device != v.device:
             raise ValueError("k and v must be CUDA tensors [pages, page_size, kv_heads, head_dim] of one shape and type")
-        if k.dtype not in (torch.float16, torch.bfloat16):
+        if dtype is not torch.float16 and dtype is not torch.bfloat16:
             raise ValueError("the cache holds fp16 or bf16")
         ks, vs = k.stride(), v.stride()
         if ks[3] != 1 or vs[3] != 1:
             raise ValueError("the cache's columns must be contiguous")
         self.k, self.v = k, v
-        pages, page, heads, dim = k.shape
-        self._c = _Cache(k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype], pages, page, heads, dim, 0,
-                         (C.c_int64 * 3)(*ks[:3]), (C.c_int64 * 3)(*vs[:3]))
+        self._c = _Cache(k.data_ptr(), v.data_ptr(), _DTYPES[dtype], *shape, 0, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2])
+        self._ref = C.byref(self._c)
 
 
 def _heads(name, x, like=None):
-    """Checks [tokens, heads, head_dim] with contiguous columns; the (token, head) strides."""
-    if x.dim() != 3 or not x.is_cuda or (x.stride(2) != 1 and x.shape[2] != 1):
+    """Checks [tokens, heads, head_dim] with contiguous columns; its address and (token, head) strides."""
+    shape, strides = x.shape, x.stride()
+    if len(shape) != 3 or not x.is_cuda or (strides[2] != 1 and shape[2] != 1):
         raise ValueError(f"{name} must be a CUDA tensor [tokens, heads, head_dim] with contiguous columns")
-    if like is not None and (x.shape[0] != like.shape[0] or x.dtype is not like.dtype or x.device != like.device):
+    if like is not None and (shape[0] != like.shape[0] or x.dtype is not like.dtype or x.device != like.device):
         raise ValueError(f"{name} must have {like.shape[0]} tokens of {like.dtype}")
-    return x.stride(0), x.stride(1)
+    return x.data_ptr(), strides[0], strides[1]
 
 
 def _table(tokens, positions, freq, axis, interleaved):
@@ -111,46 +133,43 @@ def _table(tokens, positions, freq, axis, interleaved):
     return _Table(freq.data_ptr(), axis.data_ptr(), 2 * freq.shape[0], axes, int(interleaved), 0)
 
 
+def _out(out, x):
+    if out is None:
+        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if out.shape != x.shape:
+        raise ValueError("out must have the input's shape")
+    return out
+
+
 def rope(x, positions, freq, axis, *, interleaved=False, inverse=False, out=None, stream=None):
     """Rotary positions of x [tokens, heads, head_dim] (fp32, fp16 or bf16): pair i turns by positions[:, axis[i]]
     * freq[i].  positions: int32 [tokens, axes].  inverse: turns back, the gradient of the forward rotation."""
-    xt, xh = _heads("x", x)
-    if x.dtype not in _DTYPES:
+    xp = _heads("x", x)
+    dtype = _DTYPES.get(x.dtype)
+    if dtype is None:
         raise ValueError("x must be fp32, fp16 or bf16")
-    table = _table(x.shape[0], positions, freq, axis, interleaved)
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    yt, yh = _heads("out", out, x)
-    if out.shape != x.shape:
-        raise ValueError("out must have x's shape")
-    with torch.cuda.device(x.device):
-        _check(lib().mars_rope(C.byref(table), _DTYPES[x.dtype], x.data_ptr(), xt, xh, out.data_ptr(), yt, yh,
-                               x.shape[0], x.shape[1], x.shape[2], positions.data_ptr(), int(inverse),
-                               _stream(stream, x)))
+    n, heads, dim = x.shape
+    table = _table(n, positions, freq, axis, interleaved)
+    out = _out(out, x)
+    _on_device_of(x, lib().mars_rope, (C.byref(table), dtype, *xp, *_heads("out", out, x), n, heads, dim,
+                                       positions.data_ptr(), int(inverse), _stream(stream, x)))
     return out
 
 
 def rope_append(q, k, v, positions, freq, axis, cache, slots, *, interleaved=False, out=None, stream=None):
     """q rotated (returned, or into out, which may be q), k rotated and v copied into the cache's slots.
     q: [tokens, q_heads, head_dim], k and v: [tokens, kv_heads, head_dim], all of the cache's type."""
-    qt, qh = _heads("q", q)
-    kt, kh = _heads("k", k, q)
-    vt, vh = _heads("v", v, q)
-    if q.dtype is not cache.k.dtype or k.shape[1:] != cache.k.shape[2:] or v.shape != k.shape or \
-            q.shape[2] != k.shape[2] or q.device != cache.k.device:
+    qp, kp, vp = _heads("q", q), _heads("k", k, q), _heads("v", v, q)
+    n, heads, dim = q.shape
+    c = cache._c
+    if q.dtype is not cache.k.dtype or q.device != cache.k.device or dim != c.head_dim or \
+            k.shape[1:] != (c.kv_heads, dim) or v.shape != k.shape:
         raise ValueError("q, k and v must have the cache's type, device, heads and columns")
-    table = _table(q.shape[0], positions, freq, axis, interleaved)
-    _ints("slots", slots, q.shape[0])
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ot, oh = _heads("out", out, q)
-    if out.shape != q.shape:
-        raise ValueError("out must have q's shape")
-    with torch.cuda.device(q.device):
-        _check(lib().mars_rope_append(
-            C.byref(table), C.byref(cache._c), q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
-            out.data_ptr(), ot, oh, q.shape[0], q.shape[1], positions.data_ptr(), slots.data_ptr(),
-            _stream(stream, q)))
+    table = _table(n, positions, freq, axis, interleaved)
+    slots = _ints("slots", slots, n)
+    out = _out(out, q)
+    _on_device_of(q, lib().mars_rope_append, (C.byref(table), cache._ref, *qp, *kp, *vp, *_heads("out", out, q), n, heads,
+                                              positions.data_ptr(), slots, _stream(stream, q)))
     return out
 
 
@@ -178,12 +197,10 @@ class KvContext:
     def plan(self, kv_lens, new_lens, tables, free_pages, free_count, *, page_size, max_tokens, stream=None) -> KvPlan:
         """Pages (into tables, in place), slots and positions for new_lens more tokens of each request."""
         B = kv_lens.shape[0]
-        dev = kv_lens.device
-        lens_out, count_out = torch.empty_like(kv_lens), torch.empty_like(free_count)
-        cu_new = torch.empty(B + 1, dtype=torch.int32, device=dev)
-        slots = torch.empty(max_tokens, dtype=torch.int32, device=dev)
-        positions = torch.empty(max_tokens, dtype=torch.int32, device=dev)
-        status = torch.empty(1, dtype=torch.int32, device=dev)
+        # one allocation for all that comes back
+        lens_out, cu_new, slots, positions, count_out, status = torch.empty(
+            2 * (B + max_tokens) + 3, dtype=torch.int32, device=kv_lens.device).split(
+                (B, B + 1, max_tokens, max_tokens, 1, 1))
         _check(lib().mars_kv_plan(
             self.handle, B, _ints("kv_lens", kv_lens), _ints("new_lens", new_lens, B), _ints("tables", tables, B, 2),
             tables.shape[1], page_size, _ints("free_pages", free_pages), free_pages.shape[0],
@@ -200,26 +217,23 @@ class KvContext:
         decay[head] * max(0, i - j).  max_new: the most new tokens of one request, if known (it chooses the kernel).
         Returns out (q's shape and type), with return_lse also the fp32 [tokens, q_heads] log of the scores'
         exponentials' sum."""
-        qt, qh = _heads("q", q)
-        if q.dtype is not cache.k.dtype or q.device != cache.k.device or q.shape[2] != cache._c.head_dim:
+        qp = _heads("q", q)
+        n, heads, dim = q.shape
+        if q.dtype is not cache.k.dtype or q.device != cache.k.device or dim != cache._c.head_dim:
             raise ValueError("q must have the cache's type, device and columns")
         B = kv_lens.shape[0]
-        if decay is not None and (decay.dtype is not torch.float32 or not decay.is_cuda or
-                                  not decay.is_contiguous() or decay.shape != (q.shape[1],)):
-            raise ValueError("decay must be a contiguous float32 CUDA tensor of q_heads entries")
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ot, oh = _heads("out", out, q)
-        if out.shape != q.shape:
-            raise ValueError("out must have q's shape")
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-        cfg = _Config(q.shape[2] ** -0.5 if scale is None else scale, softcap, window,
-                      q.shape[0] if max_new is None else max_new)
+        if decay is not None:
+            if decay.dtype is not torch.float32 or not decay.is_cuda or not decay.is_contiguous() or \
+                    decay.shape != (heads,):
+                raise ValueError("decay must be a contiguous float32 CUDA tensor of q_heads entries")
+            decay = decay.data_ptr()
+        out = _out(out, q)
+        lse = torch.empty((n, heads), dtype=torch.float32, device=q.device) if return_lse else None
+        cfg = _Config(dim ** -0.5 if scale is None else scale, softcap, window, n if max_new is None else max_new)
         _check(lib().mars_paged_attention(
-            self.handle, C.byref(cache._c), q.data_ptr(), qt, qh, q.shape[0], q.shape[1], B,
-            _ints("cu_new", cu_new, B + 1), _ints("kv_lens", kv_lens), _ints("tables", tables, B, 2), tables.shape[1],
-            C.byref(cfg), None if decay is None else decay.data_ptr(),
-            None if prefix_lens is None else _ints("prefix_lens", prefix_lens, B), out.data_ptr(), ot, oh,
+            self.handle, cache._ref, *qp, n, heads, B, _ints("cu_new", cu_new, B + 1), _ints("kv_lens", kv_lens),
+            _ints("tables", tables, B, 2), tables.shape[1], C.byref(cfg), decay,
+            None if prefix_lens is None else _ints("prefix_lens", prefix_lens, B), *_heads("out", out, q),
             None if lse is None else lse.data_ptr(), _stream(stream, q)))
         return (out, lse) if return_lse else out
 
