@@ -120,6 +120,7 @@ __device__ long long plan_scan(long long v, long long* total) {
 
 // starts[i]: where CTA i's share begins; starts[ctas]: the end.
 __global__ void __launch_bounds__(kPlanThreads) attn_chunk_plan_kernel(const AttnArgs a, ChunkStart* starts, int ctas) {
+    launch_dependents();                          // the main kernel sets itself up meanwhile
     extern __shared__ int s_units[];              // B: units (of one head) before request b
     const int per = kRows / a.group;
     const int each = (a.B + kPlanThreads - 1) / kPlanThreads;
@@ -274,6 +275,8 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
+    launch_dependents();
+    wait_primary();                               // the shares
 
     bool ok = true;
     if (warp < 4) {
@@ -513,18 +516,44 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
                         // the score in units of log 2 itself
                         if (a.cap > 0.0f) {
                             const float in = a.scale / a.cap, out = a.cap * kLog2e;
+                            float far = 0.0f;         // the largest |score| of the row
 #pragma unroll
-                            for (int i = 0; i < kHalf; ++i)
-                                sr[i] = __float_as_uint(out * tanh_exp(__uint_as_float(sr[i]) * in));
+                            for (int i = 0; i < kHalf; i += 2)
+                                far = fmaxf(far, fmaxf(fabsf(__uint_as_float(sr[i])), fabsf(__uint_as_float(sr[i + 1]))));
+                            if (__all_sync(0xffffffffu, far * fabsf(in) <= 0.5f)) {
+                                // cap tanh(x) = cap x P(x^2), two scores an instruction
+                                const uint64_t in2 = pair(in, in), out2 = pair(out, out);
+#pragma unroll
+                                for (int i = 0; i < kHalf; i += 2) {
+                                    const float2 e = split(tanh_small(pair(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), in2, out2));
+                                    sr[i] = __float_as_uint(e.x);
+                                    sr[i + 1] = __float_as_uint(e.y);
+                                }
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < kHalf; ++i)
+                                    sr[i] = __float_as_uint(out * tanh_exp(__uint_as_float(sr[i]) * in));
+                            }
                         } else {
 #pragma unroll
                             for (int i = 0; i < kHalf; ++i) sr[i] = __float_as_uint(__uint_as_float(sr[i]) * f);
                         }
                         if (a.decay != nullptr) {
                             const float age = (float)(pos - key0);
+                            const uint64_t rate = pair(-decay, -decay), age2 = pair(age, age);
+                            if (key0 + kHalf <= first_pos + 1) {      // no key ahead of a row
 #pragma unroll
-                            for (int i = 0; i < kHalf; ++i)
-                                sr[i] = __float_as_uint(fmaf(-decay, fmaxf(age - (float)i, 0.0f), __uint_as_float(sr[i])));
+                                for (int i = 0; i < kHalf; i += 2) {
+                                    const float2 e = split(fma2(rate, add2(age2, pair(-(float)i, -(float)(i + 1))),
+                                                                pair(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1]))));
+                                    sr[i] = __float_as_uint(e.x);
+                                    sr[i + 1] = __float_as_uint(e.y);
+                                }
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < kHalf; ++i)
+                                    sr[i] = __float_as_uint(fmaf(-decay, fmaxf(age - (float)i, 0.0f), __uint_as_float(sr[i])));
+                            }
                         }
                         f = 1.0f;
                     }
@@ -651,6 +680,7 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
 template <typename T>
 __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts,
                                                               int ctas) {
+    wait_primary();
     const int i = blockIdx.x + 1;
     const ChunkStart s = starts[i], p = starts[i - 1];
     if (s.b >= a.B || s.tile == 0) return;
@@ -679,6 +709,7 @@ __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const AttnArgs a, 
     T* out = reinterpret_cast<T*>(a.out) + (int64_t)(r.first + tok) * a.o_tok + (int64_t)head * a.o_head;
     for (int d = warp * 8; d < a.D; d += 64) {
         float v[8] = {};
+#pragma unroll 2
         for (int n = 0; n < parts; ++n) {
             const float pm = w.chunk_ml[slot(n) * 2 * kRows + row].x;
             const float f = pm == -INFINITY ? 0.0f : exp2f_fast(pm - top);
@@ -694,6 +725,24 @@ __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const AttnArgs a, 
         a.lse[(int64_t)(r.first + tok) * a.hq + head] = sum > 0.0f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
 }
 
+// Launches a kernel whose set-up may overlap the end of the one before it in the
+// stream (programmatic dependent launch; it waits for that one itself).
+template <typename... P, typename... A>
+int launch_after(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    MARS_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
+    return MARS_OK;
+}
+
 template <typename T, int kPanels, bool kFull, bool kShaped>
 int launch(const AttnArgs& a, const AttnWork& w, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
            int ctas, cudaStream_t st) {
@@ -702,12 +751,11 @@ int launch(const AttnArgs& a, const AttnWork& w, const CUtensorMap& mq, const CU
     MARS_TRY(allow_smem(reinterpret_cast<const void*>(attn_chunk_kernel<T, kPanels, kFull, kShaped>), L::kSmem, done));
     attn_chunk_plan_kernel<<<1, kPlanThreads, a.B * sizeof(int), st>>>(a, w.starts, ctas);
     MARS_CUDA_TRY(cudaGetLastError());
-    attn_chunk_kernel<T, kPanels, kFull, kShaped><<<ctas, kThreads, L::kSmem, st>>>(a, w, w.starts, mq, mk, mv);
-    MARS_CUDA_TRY(cudaGetLastError());
-    if (ctas > 1) {
-        attn_chunk_join_kernel<T><<<dim3(ctas - 1, 2 * kRows / 32), 256, 0, st>>>(a, w, w.starts, ctas);
-        MARS_CUDA_TRY(cudaGetLastError());
-    }
+    MARS_TRY(launch_after(attn_chunk_kernel<T, kPanels, kFull, kShaped>, dim3(ctas), kThreads, L::kSmem, st, a, w,
+                          (const ChunkStart*)w.starts, mq, mk, mv));
+    if (ctas > 1)
+        MARS_TRY(launch_after(attn_chunk_join_kernel<T>, dim3(ctas - 1, 2 * kRows / 32), 256, 0, st, a, w,
+                              (const ChunkStart*)w.starts, ctas));
     return MARS_OK;
 }
 

@@ -151,6 +151,32 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// out * tanh(in * s) of two scores with |in * s| <= 1/2: x P(x^2), P a polynomial
+// of degree 5 fitted here to the least largest relative error of tanh(x) / x
+// (2^-24.5 in fp32).  No special function: with two of them for a tanh and one
+// for the softmax, capped scores took three times the exponentials' time.
+__device__ __forceinline__ uint64_t tanh_small(uint64_t s, uint64_t in, uint64_t out) {
+    const uint64_t x = mul2(s, in), u = mul2(x, x);
+    uint64_t p = pair(-0.006647486239671707f, -0.006647486239671707f);
+    p = fma2(p, u, pair(0.021297989413142204f, 0.021297989413142204f));
+    p = fma2(p, u, pair(-0.053899191319942474f, -0.053899191319942474f));
+    p = fma2(p, u, pair(0.13332964479923248f, 0.13332964479923248f));
+    p = fma2(p, u, pair(-0.333333283662796f, -0.333333283662796f));
+    p = fma2(p, u, pair(1.0f, 1.0f));
+    return mul2(mul2(x, out), p);
+}
+
+// Programmatic dependent launch: the next kernel of the stream may start; wait
+// until the one before is complete and its writes are visible.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // Two values rounded to T, the first in the low half.
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {

@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~(uintptr_t)1023);
     float* s_o = reinterpret_cast<float*>(ring + kRing);
     __shared__ uint64_t s_full[L::kStages], s_empty[L::kStages];
-    __shared__ float s_m[kConsumers][kRows], s_l[kConsumers][kRows];
+    __shared__ float s_m[kConsumers][kRows], s_l[kConsumers][kRows], s_top[kRows], s_inv[kRows];
     __shared__ long long s_sum[kThreads / 32 + 1];
     __shared__ Found s_found;
     __shared__ int s_last;
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
 
         const long long at = x1 - cur.left - begin;           // the unit's place in the sequence
         const int c0 = (int)(at / share), parts = (int)((at + c - 1) / share) - c0 + 1;
-        bool write = row < valid;
+        bool write = true;
         if (parts > 1) {
             const int slot = 2 * blockIdx.x + (begin == 0);
             float* po = w.part_o + (int64_t)slot * kRows * kPartCols;
@@ -429,45 +429,64 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
                 __threadfence();
             }
             bar_sync(1, 32 * kConsumers);
-            write = write && s_last;
+            write = s_last != 0;
             if (write) {
+                // A row's eight threads take every eighth part: a cache split over all SMs
+                // has a hundred, and one after another they cost more than its reading.
+                const int r_ = min(row, valid - 1);
                 top = -INFINITY;
-                for (int p = 0; p < parts; ++p)
-                    top = fmaxf(top, __ldcg(&w.part_ml[(2 * (c0 + p) + (p == 0)) * kRows + row]).x);
+#pragma unroll 4
+                for (int p = col0; p < parts; p += 8)
+                    top = fmaxf(top, __ldcg(&w.part_ml[(2 * (c0 + p) + (p == 0)) * kRows + r_]).x);
+#pragma unroll
+                for (int off = 1; off < 8; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
                 sum = 0.0f;
-                for (int p = 0; p < parts; ++p) {
-                    const float2 ml = __ldcg(&w.part_ml[(2 * (c0 + p) + (p == 0)) * kRows + row]);
+#pragma unroll 4
+                for (int p = col0; p < parts; p += 8) {
+                    const float2 ml = __ldcg(&w.part_ml[(2 * (c0 + p) + (p == 0)) * kRows + r_]);
                     if (ml.x != -INFINITY) sum += ml.y * exp2f_fast(ml.x - top);
                 }
+#pragma unroll
+                for (int off = 1; off < 8; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
             }
         }
         if (write) {
-            const int tok = r.first + u.row0 + row / a.group, head = head0 + row % a.group;
-            const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-            T* out = reinterpret_cast<T*>(a.out) + (int64_t)tok * a.o_tok + (int64_t)head * a.o_head;
-            for (int d = col0 * 4; d < a.D; d += 32) {
+            if (col0 == 0) {
+                s_top[row] = top;
+                s_inv[row] = sum > 0.0f ? 1.0f / sum : 0.0f;
+                if (row < valid && a.lse != nullptr) {
+                    const int tok = r.first + u.row0 + row / a.group, head = head0 + row % a.group;
+                    a.lse[(int64_t)tok * a.hq + head] = sum > 0.0f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+                }
+            }
+            bar_sync(1, 32 * kConsumers);
+            // four columns of a row a thread
+            const int chunks = a.D / 4;
+            for (int i = tid; i < valid * chunks; i += 32 * kConsumers) {
+                const int orow = i / chunks, d = (i - orow * chunks) * 4;
                 float4 v;
                 if (parts > 1) {
                     v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-                    for (int p = 0; p < parts; ++p) {
-                        const int slot = 2 * (c0 + p) + (p == 0);
-                        const float pm = __ldcg(&w.part_ml[slot * kRows + row]).x;
-                        const float f = pm == -INFINITY ? 0.0f : exp2f_fast(pm - top);
-                        const float4 y = __ldcg(reinterpret_cast<const float4*>(
-                            w.part_o + ((int64_t)slot * kRows + row) * kPartCols + d));
+                    const float t0 = s_top[orow];
+#pragma unroll 8
+                    for (int p = 0; p < parts; ++p) {       // in their order: the same sum every time
+                        const int at_row = (2 * (c0 + p) + (p == 0)) * kRows + orow;
+                        const float pm = __ldcg(&w.part_ml[at_row]).x;
+                        const float4 y = __ldcg(reinterpret_cast<const float4*>(w.part_o + (int64_t)at_row * kPartCols + d));
+                        const float f = pm == -INFINITY ? 0.0f : exp2f_fast(pm - t0);
                         v.x += f * y.x;
                         v.y += f * y.y;
                         v.z += f * y.z;
                         v.w += f * y.w;
                     }
                 } else {
-                    v = *reinterpret_cast<const float4*>(s_o + row * L::kPitch + d);
+                    v = *reinterpret_cast<const float4*>(s_o + orow * L::kPitch + d);
                 }
-                *reinterpret_cast<uint2*>(out + d) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+                const float inv = s_inv[orow];
+                const int tok = r.first + u.row0 + orow / a.group, head = head0 + orow % a.group;
+                *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + (int64_t)tok * a.o_tok + (int64_t)head * a.o_head + d) =
+                    make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
             }
-            if (col0 == 0 && a.lse != nullptr)
-                a.lse[(int64_t)tok * a.hq + head] = sum > 0.0f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
         }
         bar_sync(1, 32 * kConsumers);              // s_o, s_m, s_l are the next unit's
 
