@@ -298,19 +298,17 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
                     tma_load_4d(s_q + lane * L::kPanel, &map_q, &s_qfull, (lane % kPanels) * 64, 0, k.cur.h,
                                 k.r.first + k.u.row0 + (lane / kPanels) * per);
                 const int32_t* table = a.tables + (int64_t)k.cur.b * a.pitch;
-                auto page_of = [&](int t) {           // of this lane's box; num_pages reads as 0
+                auto entry_of = [&](int t) {          // the table's, of this lane's box; -1: none
                     const int key = key_of(k.u, t) + at;
-                    int page = a.num_pages;
-                    if (on && key < k.r.len) {
-                        page = table[key / a.page];
-                        if (page < 0 || page >= a.num_pages) page = a.num_pages;
-                    }
-                    return page;
+                    return on && key < k.r.len ? table[key / a.page] : -1;
                 };
-                int page = page_of(k.begin);
+                int entry = entry_of(k.begin);
                 for (int t = k.begin; t < k.end && ok; ++t) {
-                    const int off = (key_of(k.u, t) + at) % a.page, now = page;
-    #pragma unroll
+                    // num_pages reads as 0
+                    const int off = (key_of(k.u, t) + at) % a.page;
+                    const int page = entry >= 0 && entry < a.num_pages ? entry : a.num_pages;
+                    if (t + 1 < k.end) entry = entry_of(t + 1);       // used a tile later: its latency is hidden
+#pragma unroll
                     for (int side = 0; side < 2; ++side, ++slot_no) {
                         const int slot = slot_no % L::kSlots, phase = (slot_no / L::kSlots) & 1;
                         if (slot_no >= L::kSlots && !warp_wait(&s_empty[slot], phase ^ 1, w.err, 2)) {
@@ -321,8 +319,7 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
                         __syncwarp();
                         if (on)
                             tma_load_4d(s_kv + slot * L::kSlot + panel * L::kPanel + at * 128, side == 0 ? &map_k : &map_v,
-                                        &s_full[slot], panel * 64, off, k.cur.h, now);
-                        if (side == 0 && t + 1 < k.end) page = page_of(t + 1);
+                                        &s_full[slot], panel * 64, off, k.cur.h, page);
                     }
                 }
             }
