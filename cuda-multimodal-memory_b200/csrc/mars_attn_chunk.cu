@@ -95,7 +95,7 @@ __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xfffffff
 
 // ---- shares -----------------------------------------------------------------
 
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 256;
 
 __device__ long long plan_scan(long long v, long long* total) {
     __shared__ long long s_sum[kPlanThreads / 32];
