@@ -32,7 +32,7 @@ using namespace mars;
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;              // of a block at most
 constexpr int kMaxTokens = 4;          // tokens of one block
 constexpr int kMaxHalf = 512;          // pairs of a head
 
@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeArgs a) {
     const int n = (int)min((int64_t)a.tokens_per_block, a.T - t0);
     const int tid = threadIdx.y * blockDim.x + threadIdx.x;
 
-    for (int i = tid; i < n * a.half; i += kThreads) {
+    for (int i = tid; i < n * a.half; i += blockDim.x * blockDim.y) {
         const int t = i / a.half, p = i - t * a.half;
         const int ax = min(max(a.axis[p], 0), a.axes - 1);
         const double turns = (double)a.positions[(t0 + t) * a.axes + ax] * (double)a.freq[p] * 0.31830988618379067154;
@@ -177,7 +177,11 @@ void launch(const RopeArgs& a, bool interleaved, cudaStream_t st) {
     const int items = std::max(1, (a.D / V + 1) / 2);      // of one head
     int x = 1;
     while (x < items && x < 32) x *= 2;
-    const dim3 block(x, kThreads / x);
+    // Half the threads where a token has few items: the blocks' angles and loads
+    // overlap better (12 heads of 64 columns in fp32: 23.1 us with 256, 20.6 with
+    // 128; 48 heads of 128 in bf16: 41.1 and 45.3).
+    const int threads = items * (a.hq + 2 * a.hkv) <= 128 ? kThreads / 2 : kThreads;
+    const dim3 block(x, threads / x);
     const unsigned grid = (unsigned)((a.T + a.tokens_per_block - 1) / a.tokens_per_block);
     const size_t smem = (size_t)a.tokens_per_block * a.half * sizeof(float2);
     if (interleaved) rope_kernel<T, V, true><<<grid, block, smem, st>>>(a);
