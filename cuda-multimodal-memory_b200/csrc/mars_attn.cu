@@ -107,6 +107,8 @@ extern "C" int mars_paged_attention(mars_kv_ctx* c, const mars_kv_cache* cache, 
     if (cache->head_dim % 8 != 0 || cache->head_dim > MARS_ATTN_MAX_HEAD_DIM || cache->page_size % 8 != 0)
         return fail(MARS_ERR_UNSUPPORTED, fn + ": head_dim must be a multiple of 8 up to " +
                                               std::to_string(MARS_ATTN_MAX_HEAD_DIM) + ", page_size a multiple of 8");
+    if ((int64_t)cache->num_pages * cache->page_size > MARS_ATTN_MAX_KEYS)
+        return fail(MARS_ERR_UNSUPPORTED, fn + ": at most " + std::to_string(MARS_ATTN_MAX_KEYS) + " tokens a cache");
     if (q_heads / cache->kv_heads > MARS_ATTN_MAX_GROUP)
         return fail(MARS_ERR_UNSUPPORTED, fn + ": at most " + std::to_string(MARS_ATTN_MAX_GROUP) + " query heads a key head");
     if (!std::isfinite(cfg->scale) || !(cfg->softcap >= 0.0f) || !std::isfinite(cfg->softcap) || cfg->window < 0)
@@ -141,10 +143,15 @@ extern "C" int mars_paged_attention(mars_kv_ctx* c, const mars_kv_cache* cache, 
     a.scale = cfg->scale; a.cap = cfg->softcap; a.window = cfg->window;
     a.T = tokens; a.B = B; a.hq = q_heads; a.hkv = cache->kv_heads; a.group = q_heads / cache->kv_heads;
     a.D = cache->head_dim; a.page = cache->page_size; a.num_pages = cache->num_pages; a.pitch = table_pitch;
+    // The short kernel's tiles have 16 rows; more rows would read the keys once for
+    // every 16, the chunk kernel once for every 256 (which a single row takes 22 us
+    // for at the least, the short kernel 10).
+    const bool chunk = (int64_t)std::max(cfg->max_new, 1) * a.group > kShortRows;
+    MARS_TRY(kv_attn_memory(c, chunk));
     AttnWork w{};
     w.part_o = c->d_part_o; w.part_ml = c->d_part_ml; w.tickets = c->d_tickets + kKvTickets; w.err = c->d_err;
     w.host_err = c->h_err; w.chunk_o = c->d_chunk_o; w.chunk_ml = c->d_chunk_ml; w.starts = c->d_starts;
-    if ((int64_t)std::max(cfg->max_new, 1) * a.group <= kShortRows) {
+    if (!chunk) {
         MARS_TRY(attn_short(a, w, cache, c->num_sms, st));
         return kv_end(c, st);
     }

@@ -14,6 +14,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "mars_b200.h"
+
 namespace mars {
 
 struct AttnArgs {
@@ -44,7 +46,8 @@ __device__ __forceinline__ Request load_request(const AttnArgs& a, int b) {
     Request r;
     r.first = min(max(a.cu_new[b], 0), a.T);
     r.rows = min(max(a.cu_new[b + 1], r.first), a.T) - r.first;
-    r.len = (int)min((int64_t)max(a.kv_lens[b], 0), (int64_t)a.pitch * a.page);
+    // (keys are counted in 32 bits, tiles past the last one included)
+    r.len = (int)min((int64_t)max(a.kv_lens[b], 0), min((int64_t)a.pitch * a.page, (int64_t)MARS_ATTN_MAX_KEYS));
     r.prefix = a.prefix != nullptr ? min(max(a.prefix[b], 0), r.len) : 0;
     return r;
 }

@@ -28,10 +28,20 @@
 //
 // Work is shared as in mars_attn_short.cu: the units' tiles in one sequence,
 // an equal share for each CTA.  A one-block kernel before it finds the shares
-// (prompts have thousands of units), a kernel after it joins cut units.
+// (prompts have thousands of units), a kernel after it joins cut units; their
+// set-ups overlap (programmatic dependent launch).
 //
-// Bound: the tensor cores and the exponentials, which are even here: 128 x 128
-// scores take 1,024 cycles of products at D = 128 and 1,024 of ex2.
+// Bound: 64 keys of the two row tiles take 1,280 cycles of products at D = 128
+// (S 16 x 48, read from shared memory at its full rate; O 8 x 64) and 1,024 of
+// exponentials (16 ex2 a cycle), measured alone; together a step takes 1,900
+// to 2,100, what is left being the way from weights to the next scores there
+// and back (arrive, product, commit, wait: 1,700 cycles) and both warpgroups
+// at their exponentials at once.  Measured: two prompts of 8,192 and 4,142
+// tokens, 32 heads on 8 of 128 columns, 843 us = 838 TFLOP/s at 1.55 GHz under
+// the power cap (the library's sustained rate for a plain product: 1,398).
+// Tried and dropped: exponentials on the FMA units beside the special function
+// unit (slower: 8 FMA cycles an element against 8 of ex2), the warpgroups held
+// out of step, one buffer of 128 keys' scores (915 us).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -24,6 +24,11 @@
 //    of which decoding would fill 1 to 16.  The scores' registers are the
 //    second product's operand as they stand.  Rate: 512 of the 2,800 cycles
 //    that a 128-key tile takes from HBM.
+//
+// Measured (bf16, D = 128): 64 requests of up to 8,000 keys, 32 heads on 8:
+// 207 us, 6.09 TB/s, 0.95 of the copy rate.  2 requests of up to 250,000, 16
+// heads on 4: 137 us, 0.87; there a unit is cut into 74 parts, and its joining
+// is what the other has not (it was 156 us with one thread a row to join).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -11,7 +11,8 @@
 //
 // Both kernels do next to no arithmetic and move 4 to 12 bytes for each token
 // and page; what bounds them is the launch and the chain lengths -> prefix sum
-// -> page id -> slot.  So every block forms the prefix sums of all requests by
+// -> page id -> slot (3 to 8 us on the device; a call from Python takes 19 us,
+// its host time).  So every block forms the prefix sums of all requests by
 // itself (at most 8,192 of them, 64 KB from L2) instead of waiting for another
 // launch, and finds a token's request by bisection in shared memory.  Inputs
 // and outputs may be the same arrays: the last block to arrive (a counter, no
@@ -19,14 +20,59 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <mutex>
 #include <string>
+#include <vector>
 
 #include "mars_attn_mma.cuh"
 #include "mars_kv.h"
 
 using namespace mars;
 
+namespace {
+
+// Words of pinned host memory, one for each context: a page for all of them
+// (pinning one costs more than the rest of a context's creation).
+std::mutex g_words_lock;
+std::vector<int*> g_words;
+
+int host_word(int** out) {
+    std::lock_guard<std::mutex> lock(g_words_lock);
+    if (g_words.empty()) {
+        constexpr int kWords = 512;
+        int* page = nullptr;
+        MARS_CUDA_TRY(cudaHostAlloc(&page, kWords * sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable));
+        for (int i = 0; i < kWords; ++i) g_words.push_back(page + i);
+    }
+    *out = g_words.back();
+    g_words.pop_back();
+    return MARS_OK;
+}
+
+void free_host_word(int* w) {
+    std::lock_guard<std::mutex> lock(g_words_lock);
+    g_words.push_back(w);
+}
+
+}  // namespace
+
 namespace mars {
+
+int kv_attn_memory(mars_kv_ctx* c, bool chunk) {
+    const size_t sms = (size_t)c->num_sms;
+    if (!chunk && c->d_part_ml == nullptr) {
+        const size_t slots = 2 * 2 * sms;          // two of each CTA, two CTAs an SM
+        if (c->d_part_o == nullptr) MARS_CUDA_TRY(cudaMalloc(&c->d_part_o, slots * kShortRows * kPartCols * sizeof(float)));
+        MARS_CUDA_TRY(cudaMalloc(&c->d_part_ml, slots * kShortRows * sizeof(float2)));
+    }
+    if (chunk && c->d_starts == nullptr) {
+        const size_t rows = 256, slots = 2 * sms;
+        if (c->d_chunk_o == nullptr) MARS_CUDA_TRY(cudaMalloc(&c->d_chunk_o, slots * rows * kPartCols * sizeof(float)));
+        if (c->d_chunk_ml == nullptr) MARS_CUDA_TRY(cudaMalloc(&c->d_chunk_ml, slots * rows * sizeof(float2)));
+        MARS_CUDA_TRY(cudaMalloc(&c->d_starts, (sms + 1) * sizeof(ChunkStart)));
+    }
+    return MARS_OK;
+}
 
 int kv_begin(mars_kv_ctx* c, void* stream, cudaStream_t* st) {
     if (*static_cast<volatile int*>(c->h_err) != 0) {
@@ -144,7 +190,6 @@ struct ReleaseArgs {
 };
 
 // Pages of the flagged requests onto the free stack, request by request.
-// Measured: in the table of the plan kernel below.
 __global__ void __launch_bounds__(kThreads) kv_release_kernel(const ReleaseArgs a) {
     extern __shared__ int32_t s_first[];           // B: released pages before request b
     const int per = (a.B + kThreads - 1) / kThreads;
@@ -310,16 +355,10 @@ extern "C" int mars_kv_ctx_create(int32_t device, int32_t max_requests, mars_kv_
     auto build = [&]() -> int {
         MARS_CUDA_TRY(cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking));
         MARS_CUDA_TRY(cudaEventCreateWithFlags(&c->used, cudaEventDisableTiming));
-        const size_t ctas = 2 * (size_t)sms, slots = 2 * ctas, words = kKvTickets + ctas + 1;
+        const size_t words = kKvTickets + 2 * (size_t)sms + 1;
         MARS_CUDA_TRY(cudaMalloc(&c->d_tickets, words * sizeof(unsigned int)));
-        c->d_err = reinterpret_cast<int*>(c->d_tickets + kKvTickets + ctas);
-        MARS_CUDA_TRY(cudaMalloc(&c->d_part_o, slots * kShortRows * kPartCols * sizeof(float)));
-        MARS_CUDA_TRY(cudaMalloc(&c->d_part_ml, slots * kShortRows * sizeof(float2)));
-        const size_t chunk_rows = 256, chunk_slots = 2 * (size_t)sms;
-        MARS_CUDA_TRY(cudaMalloc(&c->d_chunk_o, chunk_slots * chunk_rows * kPartCols * sizeof(float)));
-        MARS_CUDA_TRY(cudaMalloc(&c->d_chunk_ml, chunk_slots * chunk_rows * sizeof(float2)));
-        MARS_CUDA_TRY(cudaMalloc(&c->d_starts, ((size_t)sms + 1) * sizeof(ChunkStart)));
-        MARS_CUDA_TRY(cudaHostAlloc(&c->h_err, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable));
+        c->d_err = reinterpret_cast<int*>(c->d_tickets + kKvTickets + 2 * (size_t)sms);
+        MARS_TRY(host_word(&c->h_err));
         *c->h_err = 0;
         MARS_CUDA_TRY(cudaMemsetAsync(c->d_tickets, 0, words * sizeof(unsigned int), c->stream));
         // the largest context's: the attribute is the device's, not the context's
@@ -347,7 +386,7 @@ extern "C" int mars_kv_ctx_destroy(mars_kv_ctx* c) {
     if (c->d_chunk_o != nullptr) cudaFree(c->d_chunk_o);
     if (c->d_chunk_ml != nullptr) cudaFree(c->d_chunk_ml);
     if (c->d_starts != nullptr) cudaFree(c->d_starts);
-    if (c->h_err != nullptr) cudaFreeHost(c->h_err);
+    if (c->h_err != nullptr) free_host_word(c->h_err);
     if (c->used != nullptr) cudaEventDestroy(c->used);
     if (c->stream != nullptr) cudaStreamDestroy(c->stream);
     delete c;

@@ -46,6 +46,8 @@ constexpr int kTicketRelease = 0;
 constexpr int kTicketPlan = 1;
 constexpr int kKvTickets = 2;
 
+// The attention kernels' parts (5 or 39 MB), made by the first call of each kind.
+int kv_attn_memory(mars_kv_ctx* c, bool chunk);
 // The stream of a call on `c`, ordered after the context's previous call.
 int kv_begin(mars_kv_ctx* c, void* stream, cudaStream_t* st);
 // Marks the end of the call's work on `st`.

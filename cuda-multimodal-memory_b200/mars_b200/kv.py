@@ -182,9 +182,14 @@ class KvContext:
         self.handle = h
         self.device = device
 
+    def _here(self, t):
+        if t.get_device() != self.device:
+            raise ValueError(f"the context works on device {self.device}, a tensor is on {t.device}")
+
     def release(self, kv_lens, finished, tables, free_pages, free_count, *, page_size, status=None, stream=None):
         """Push the pages of the requests with finished != 0 onto the free stack; returns the new
         (kv_lens, free_count).  A failure (status, one int32, if given) leaves everything as it was."""
+        self._here(kv_lens)
         B = kv_lens.shape[0]
         lens_out, count_out = torch.empty_like(kv_lens), torch.empty_like(free_count)
         _check(lib().mars_kv_release(
@@ -196,6 +201,7 @@ class KvContext:
 
     def plan(self, kv_lens, new_lens, tables, free_pages, free_count, *, page_size, max_tokens, stream=None) -> KvPlan:
         """Pages (into tables, in place), slots and positions for new_lens more tokens of each request."""
+        self._here(kv_lens)
         B = kv_lens.shape[0]
         # one allocation for all that comes back
         lens_out, cu_new, slots, positions, count_out, status = torch.empty(
@@ -221,6 +227,7 @@ class KvContext:
         n, heads, dim = q.shape
         if q.dtype is not cache.k.dtype or q.device != cache.k.device or dim != cache._c.head_dim:
             raise ValueError("q must have the cache's type, device and columns")
+        self._here(q)
         B = kv_lens.shape[0]
         if decay is not None:
             if decay.dtype is not torch.float32 or not decay.is_cuda or not decay.is_contiguous() or \

@@ -600,7 +600,9 @@ int mars_scan_topk_noalloc(const float* d_embeddings, int32_t row_pitch,
 #define MARS_KV_MAX_REQUESTS 8192
 typedef struct mars_kv_ctx mars_kv_ctx;
 
-/* Working memory for calls of up to max_requests requests. */
+/* Working memory for calls of up to max_requests requests.  The attention's
+ * (5 MB for few new tokens, 39 MB for chunks) is made by its first call of each
+ * kind, which for that reason must not be inside a stream capture. */
 int mars_kv_ctx_create(int32_t device, int32_t max_requests, mars_kv_ctx** out);
 /* Waits for the context's last call.  NULL is accepted. */
 int mars_kv_ctx_destroy(mars_kv_ctx* ctx);
@@ -719,8 +721,12 @@ int mars_rope_append(const mars_rope_table* table, const mars_kv_cache* cache, c
  * influence, non-finite values included; of the keys below the length, the
  * values must be finite.  A table entry outside [0, num_pages) reads as zero
  * keys and values.
+ * A bounded device wait that gave up is returned as MARS_ERR_TIMEOUT by the
+ * context's next call; the call it happened in has no valid results.
  * Limits: head_dim a multiple of 8 up to 128, page_size a multiple of 8, at
- * most 128 query heads a key head; all rows on 16-byte boundaries. */
+ * most 128 query heads a key head, at most MARS_ATTN_MAX_KEYS keys a request;
+ * all rows on 16-byte boundaries. */
+#define MARS_ATTN_MAX_KEYS 2147482624
 #define MARS_ATTN_MAX_HEAD_DIM 128
 #define MARS_ATTN_MAX_GROUP 128
 typedef struct mars_attn_config {
