@@ -143,9 +143,10 @@ extern "C" int mars_paged_attention(mars_kv_ctx* c, const mars_kv_cache* cache, 
     a.scale = cfg->scale; a.cap = cfg->softcap; a.window = cfg->window;
     a.T = tokens; a.B = B; a.hq = q_heads; a.hkv = cache->kv_heads; a.group = q_heads / cache->kv_heads;
     a.D = cache->head_dim; a.page = cache->page_size; a.num_pages = cache->num_pages; a.pitch = table_pitch;
-    // The short kernel's tiles have 16 rows; more rows would read the keys once for
-    // every 16, the chunk kernel once for every 256 (which a single row takes 22 us
-    // for at the least, the short kernel 10).
+    // The short kernel's tiles have 16 rows: with more it would read the keys once for
+    // every 16, the chunk kernel once for every 256 but with three launches and tiles
+    // of 128 rows (64 ragged requests, 4 query heads a key head: 4 new tokens 202 us
+    // here, 5 there 259; 4 requests of 700 keys: 14 us and 18).
     const bool chunk = (int64_t)std::max(cfg->max_new, 1) * a.group > kShortRows;
     MARS_TRY(kv_attn_memory(c, chunk));
     AttnWork w{};
