@@ -12,7 +12,7 @@
 //             of row tile 1  [256,384) O0  [384,512) O1
 //
 // While a warpgroup works on one half, the other half's weights are multiplied
-// and the next scores are made there, so it never waits for the tensor cores:
+// and the next scores are made there, so it has scores to go on with:
 // with scores of 128 keys at once (one buffer) each tile was a chain softmax ->
 // O -> next S of 5,000 cycles for 2,048 cycles of products.
 // The running maximum that P is scaled by follows the true one only when it
