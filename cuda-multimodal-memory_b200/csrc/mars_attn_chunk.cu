@@ -490,6 +490,7 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
         const int t = (warp - 4) >> 2, row = tid - 128 - t * 128;
         const uint32_t tm_s = tmem + ((uint32_t)(warp & 3) << 21) + t * 128;      // lanes of this warp
         const uint32_t tm_o = tm_s + 256;
+        const SmallTanh small = kShaped && a.cap > 0.0f ? small_tanh(a.scale / a.cap, a.cap * kLog2e) : SmallTanh{};
         int seen_tiles = 0;                       // the phase of each half's barriers
         for (; more && ok; more = k.next(a, per)) {
             if (t >= k.u.nq) continue;
@@ -526,13 +527,12 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
                             float far = 0.0f;         // the largest |score| of the row
 #pragma unroll
                             for (int i = 0; i < kHalf; i += 2)
-                                far = fmaxf(far, fmaxf(fabsf(__uint_as_float(sr[i])), fabsf(__uint_as_float(sr[i + 1]))));
-                            if (__all_sync(0xffffffffu, far * fabsf(in) <= 0.5f)) {
-                                // cap tanh(x) = cap x P(x^2), two scores an instruction
-                                const uint64_t in2 = pair(in, in), out2 = pair(out, out);
+                                far = max3(far, fabsf(__uint_as_float(sr[i])), fabsf(__uint_as_float(sr[i + 1])));
+                            if (__all_sync(0xffffffffu, far * fabsf(in) <= 0.5f && far < 1e18f)) {      // its square is finite
+                                // two scores an instruction
 #pragma unroll
                                 for (int i = 0; i < kHalf; i += 2) {
-                                    const float2 e = split(tanh_small(pair(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), in2, out2));
+                                    const float2 e = split(tanh_small(pair(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), small));
                                     sr[i] = __float_as_uint(e.x);
                                     sr[i + 1] = __float_as_uint(e.y);
                                 }

@@ -157,19 +157,32 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
     return r;
 }
 
-// out * tanh(in * s) of two scores with |in * s| <= 1/2: x P(x^2), P a polynomial
-// of degree 5 fitted here to the least largest relative error of tanh(x) / x
-// (2^-24.5 in fp32).  No special function: with two of them for a tanh and one
-// for the softmax, capped scores took three times the exponentials' time.
-__device__ __forceinline__ uint64_t tanh_small(uint64_t s, uint64_t in, uint64_t out) {
-    const uint64_t x = mul2(s, in), u = mul2(x, x);
-    uint64_t p = pair(-0.006647486239671707f, -0.006647486239671707f);
-    p = fma2(p, u, pair(0.021297989413142204f, 0.021297989413142204f));
-    p = fma2(p, u, pair(-0.053899191319942474f, -0.053899191319942474f));
-    p = fma2(p, u, pair(0.13332964479923248f, 0.13332964479923248f));
-    p = fma2(p, u, pair(-0.333333283662796f, -0.333333283662796f));
-    p = fma2(p, u, pair(1.0f, 1.0f));
-    return mul2(mul2(x, out), p);
+// out * tanh(in * s) for |in * s| <= 1/2 as s P(s^2), P a polynomial of degree 5
+// fitted here to the least largest relative error of tanh(x) / x (2^-24.5 in
+// fp32), its coefficients taking the powers of in and out.  No special function:
+// with two of them for a tanh and one for the softmax, capped scores took three
+// times the exponentials' time.
+struct SmallTanh {
+    float c[6];
+};
+__device__ __forceinline__ SmallTanh small_tanh(float in, float out) {
+    const float fit[6] = {1.0f, -0.333333283662796f, 0.13332964479923248f, -0.053899191319942474f, 0.021297989413142204f,
+                          -0.006647486239671707f};
+    SmallTanh t;
+    float power = in * out;
+#pragma unroll
+    for (int k = 0; k < 6; ++k) {
+        t.c[k] = fit[k] * power;
+        power *= in * in;
+    }
+    return t;
+}
+__device__ __forceinline__ uint64_t tanh_small(uint64_t s, const SmallTanh& t) {
+    const uint64_t u = mul2(s, s);
+    uint64_t p = pair(t.c[5], t.c[5]);
+#pragma unroll
+    for (int k = 4; k >= 0; --k) p = fma2(p, u, pair(t.c[k], t.c[k]));
+    return mul2(s, p);
 }
 
 // Programmatic dependent launch: the next kernel of the stream may start; wait
