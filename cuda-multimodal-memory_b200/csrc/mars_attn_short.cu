@@ -7,7 +7,7 @@
 // TMA loads with as little as possible between them.
 //
 //  * Split.  The work is the sequence of all (request, row tile, key head)
-//    units' 64-key tiles; every CTA takes an equal share of that sequence, as
+//    units' tiles of keys; every CTA takes an equal share of that sequence, as
 //    many shares as CTAs fit the card.  Any mix of lengths is balanced to one
 //    tile, a long cache is split over all SMs and short ones share a CTA.  The
 //    shares follow from the lengths alone, which every CTA sums up by itself
@@ -17,7 +17,7 @@
 //    the result does not depend on timing.
 //  * Pipeline.  One producer warp, a lane for each box of a page, fills a ring
 //    of 96 KB (two CTAs an SM: 192 KB in flight, three times what latency x
-//    bandwidth asks for).  Four consumer warps take 16 keys of a tile each and
+//    bandwidth asks for).  Four consumer warps take a quarter of a tile's keys each and
 //    keep a running maximum, sum and accumulator of their own, so nothing but
 //    the ring's barriers joins them before a unit's end.
 //  * mma.sync m16n8k16.  16 rows are one of its tiles; a tcgen05 tile has 128,
@@ -45,13 +45,17 @@ using namespace mars::sm100;
 
 namespace {
 
-constexpr int kTile = 64;                       // keys
 constexpr int kRows = kShortRows;               // 16
 constexpr int kConsumers = 4;                   // warps
 constexpr int kThreads = 32 * (kConsumers + 1);
 constexpr int kRing = 96 * 1024;
 
+// A tile is 32 KB of keys and values: 128 keys of up to 64 columns, 64 of up to
+// 128.  (64 keys of 64 columns, 16 KB, left what a tile costs beside its bytes
+// -- barriers, masks, maxima, rescaling -- in the way: 4.0 TB/s.)
 template <int kPanels> struct Layout {
+    static constexpr int kTile = 128 / kPanels;                   // keys
+    static constexpr int kPer = kTile / kConsumers;               // of a warp: 32 or 16
     static constexpr int kStage = 2 * kPanels * kTile * 128;      // bytes: keys, then values
     static constexpr int kStages = kRing / kStage;
     static constexpr int kCols = 64 * kPanels;
@@ -66,6 +70,7 @@ struct Unit {
     int low, high;                // the rest's keys
 };
 
+template <int kTile>
 __device__ __forceinline__ Unit make_unit(const AttnArgs& a, const Request& r, int qt, int per) {
     Unit u;
     u.row0 = qt * per;
@@ -90,6 +95,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
                                                                  const __grid_constant__ CUtensorMap map_k,
                                                                  const __grid_constant__ CUtensorMap map_v) {
     using L = Layout<kPanels>;
+    constexpr int kTile = L::kTile, kBlocks = L::kPer / 8;        // blocks of 8 keys a warp
     extern __shared__ uint8_t s_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~(uintptr_t)1023);
     float* s_o = reinterpret_cast<float*>(ring + kRing);
@@ -117,7 +123,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
     long long mine = 0;
     for (int b = b0; b < b1; ++b) {
         const Request r = load_request(a, b);
-        for (int qt = 0; qt * per < r.rows; ++qt) mine += max(1, make_unit(a, r, qt, per).tiles);
+        for (int qt = 0; qt * per < r.rows; ++qt) mine += max(1, make_unit<kTile>(a, r, qt, per).tiles);
     }
     mine *= a.hkv;
     long long upto = mine;
@@ -142,7 +148,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
         for (int b = b0; b < b1; ++b) {
             const Request r = load_request(a, b);
             for (int qt = 0; qt * per < r.rows; ++qt) {
-                const int c = max(1, make_unit(a, r, qt, per).tiles);
+                const int c = max(1, make_unit<kTile>(a, r, qt, per).tiles);
                 if (x >= 0 && x < (long long)c * a.hkv)
                     s_found = Found{b, qt, (int)(x / c), (int)(x % c)};
                 x -= (long long)c * a.hkv;
@@ -166,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
         int issued = 0;
         bool ok = true;
         while (ok && cur.left > 0) {
-            const Unit u = make_unit(a, r, cur.qt, per);
+            const Unit u = make_unit<kTile>(a, r, cur.qt, per);
             const int c = max(1, u.tiles), end = (int)min((long long)c, cur.tile + cur.left);
             const int32_t* table = a.tables + (int64_t)cur.b * a.pitch;
             auto page_of = [&](int t) {           // of this lane's box in tile t of the unit; num_pages: reads as 0
@@ -214,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
     int used = 0;
     bool ok = true;
     while (cur.left > 0) {
-        const Unit u = make_unit(a, r, cur.qt, per);
+        const Unit u = make_unit<kTile>(a, r, cur.qt, per);
         const int c = max(1, u.tiles), begin = cur.tile, end = (int)min((long long)c, begin + cur.left);
         const int head0 = cur.h * a.group, valid = u.rows * a.group;
 
@@ -257,21 +263,25 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
             // a wait that gave up: the unit's barriers are still taken, so that no warp is left at one
             ok = ok && warp_wait(&s_full[stage], (used / L::kStages) & 1, w.err, 3);
             if (!ok) continue;
-            const int key0 = (t < u.n1 ? t : u.s2 + t - u.n1) * kTile + warp * 16;
-            const uint32_t sk = smem_u32(ring + stage * L::kStage) + warp * 16 * 128;
+            const int key0 = (t < u.n1 ? t : u.s2 + t - u.n1) * kTile + warp * L::kPer;
+            const uint32_t sk = smem_u32(ring + stage * L::kStage) + warp * L::kPer * 128;
             const uint32_t sv = sk + kPanels * kTile * 128;
 
-            // scores of 16 keys: two blocks of 8
-            float s[2][4] = {};
+            // scores of the warp's keys, blocks of 8
+            float s[kBlocks][4] = {};
             {
                 const int row = lane & 7, tok = ((lane >> 4) << 3) + row, half = (lane >> 3) & 1;
 #pragma unroll
                 for (int ks = 0; ks < 4 * kPanels; ++ks) {
                     if (ks * 16 < a.D) {
-                        uint32_t f[4];
-                        ldmatrix_x4(f, sk + (ks >> 2) * kTile * 128 + tok * 128 + ((((ks & 3) * 2 + half) ^ row) << 4));
-                        mma_16816<T>(s[0], qf[ks], f[0], f[1]);
-                        mma_16816<T>(s[1], qf[ks], f[2], f[3]);
+#pragma unroll
+                        for (int x = 0; x < kBlocks / 2; ++x) {
+                            uint32_t f[4];
+                            ldmatrix_x4(f, sk + (ks >> 2) * kTile * 128 + (x * 16 + tok) * 128 +
+                                               ((((ks & 3) * 2 + half) ^ row) << 4));
+                            mma_16816<T>(s[2 * x], qf[ks], f[0], f[1]);
+                            mma_16816<T>(s[2 * x + 1], qf[ks], f[2], f[3]);
+                        }
                     }
                 }
             }
@@ -279,41 +289,44 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
             if (a.cap > 0.0f) {
                 const float in = a.scale / a.cap, out = a.cap * kLog2e;
 #pragma unroll
-                for (int nb = 0; nb < 2; ++nb)
+                for (int nb = 0; nb < kBlocks; ++nb)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[nb][e] = out * tanh_exp(s[nb][e] * in);
             } else {
                 const float f = a.scale * kLog2e;
 #pragma unroll
-                for (int nb = 0; nb < 2; ++nb)
+                for (int nb = 0; nb < kBlocks; ++nb)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[nb][e] *= f;
             }
             if (a.decay != nullptr) {
 #pragma unroll
-                for (int nb = 0; nb < 2; ++nb)
+                for (int nb = 0; nb < kBlocks; ++nb)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         s[nb][e] -= decay[e >> 1] * (float)max(0, pos[e >> 1] - (key0 + nb * 8 + qc + (e & 1)));
             }
-            const bool all = key0 + 16 <= r.prefix || (key0 >= all_lo && key0 + 16 <= all_hi);
+            const bool all = key0 + L::kPer <= r.prefix || (key0 >= all_lo && key0 + L::kPer <= all_hi);
             if (!all) {
 #pragma unroll
-                for (int nb = 0; nb < 2; ++nb)
+                for (int nb = 0; nb < kBlocks; ++nb)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int j = key0 + nb * 8 + qc + (e & 1), i = e >> 1;
                         if (!(j < pre[i] || (j >= lo[i] && j < hi[i]))) s[nb][e] = -INFINITY;
                     }
                 // Values of keys that no row sees may be anything, and 0 x NaN is
-                // NaN: put zeros there (each lane half a row of one panel's 128 B).
-                const int j = key0 + (lane >> 1);
-                if (!(j < r.prefix || (j >= u.low && j < u.high))) {
+                // NaN: put zeros there (a lane half a row of one panel's 128 B).
 #pragma unroll
-                    for (int p = 0; p < kPanels; ++p)
+                for (int half = lane; half < 2 * L::kPer; half += 32) {
+                    const int j = key0 + (half >> 1);
+                    if (!(j < r.prefix || (j >= u.low && j < u.high))) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            st_shared_zero16(sv + p * kTile * 128 + (lane >> 1) * 128 + (lane & 1) * 64 + i * 16);
+                        for (int p = 0; p < kPanels; ++p)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                st_shared_zero16(sv + p * kTile * 128 + (half >> 1) * 128 + (half & 1) * 64 + i * 16);
+                    }
                 }
                 fence_proxy_async();               // before the ring's next TMA write of this stage
                 __syncwarp();
@@ -323,7 +336,9 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
             bool moved = false;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                float x = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
+                float x = fmaxf(s[0][2 * i], s[0][2 * i + 1]);
+#pragma unroll
+                for (int nb = 1; nb < kBlocks; ++nb) x = max3(x, s[nb][2 * i], s[nb][2 * i + 1]);
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
                 x = fmaxf(x, m[i]);
@@ -344,16 +359,18 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
             }
             const float base[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
 #pragma unroll
-            for (int nb = 0; nb < 2; ++nb)
+            for (int nb = 0; nb < kBlocks; ++nb)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     s[nb][e] = exp2f_fast(s[nb][e] - base[e >> 1]);
                     l[e >> 1] += s[nb][e];
                 }
-            uint32_t pf[4] = {pack2<T>(s[0][0], s[0][1]), pack2<T>(s[0][2], s[0][3]), pack2<T>(s[1][0], s[1][1]),
-                              pack2<T>(s[1][2], s[1][3])};
-            {
-                const int row = lane & 7, tok = (((lane >> 3) & 1) << 3) + row, half = lane >> 4;
+#pragma unroll
+            for (int x = 0; x < kBlocks / 2; ++x) {
+                const float(&s0)[4] = s[2 * x], (&s1)[4] = s[2 * x + 1];
+                const uint32_t pf[4] = {pack2<T>(s0[0], s0[1]), pack2<T>(s0[2], s0[3]), pack2<T>(s1[0], s1[1]),
+                                        pack2<T>(s1[2], s1[3])};
+                const int row = lane & 7, tok = x * 16 + (((lane >> 3) & 1) << 3) + row, half = lane >> 4;
 #pragma unroll
                 for (int db = 0; db < 4 * kPanels; ++db) {
                     if (db * 16 < a.D) {
@@ -524,12 +541,12 @@ namespace mars {
 
 int attn_short(const AttnArgs& a, AttnWork w, const mars_kv_cache* cache, int num_sms, cudaStream_t st) {
     CUtensorMap mk, mv;
-    w.box = page_box(cache->page_size, kTile);
+    w.box = page_box(cache->page_size, a.D <= 64 ? Layout<1>::kTile : Layout<2>::kTile);
     MARS_TRY(page_maps(cache, w.box, &mk, &mv));
-    // Small calls: 2 tiles a CTA.  A piece costs 2 to 3 us beside its tiles (its rows'
+    // Small calls: 128 keys a CTA.  A piece costs 2 to 3 us beside its tiles (its rows'
     // queries, the warps' joining, the output), so fewer and larger shares are slower
     // (1 request of 100 keys, 12 heads: 7.4 us with 2, 11.0 with 4, 25.5 with 12).
-    w.min_share = 2;
+    w.min_share = a.D <= 64 ? 1 : 2;
     if (cache->dtype == MARS_DTYPE_F16)
         return a.D <= 64 ? launch<__half, 1>(a, w, mk, mv, num_sms, st) : launch<__half, 2>(a, w, mk, mv, num_sms, st);
     return a.D <= 64 ? launch<__nv_bfloat16, 1>(a, w, mk, mv, num_sms, st)
