@@ -48,13 +48,18 @@ int page_maps(const mars_kv_cache* c, int box, CUtensorMap* k, CUtensorMap* v) {
     const cuuint32_t shape[4] = {64, (cuuint32_t)box, 1, 1}, unit[4] = {1, 1, 1, 1};
     const CUtensorMapDataType type =
         c->dtype == MARS_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    // A key is one piece of memory; where it is 128 bytes, fetching 256 would read its
+    // neighbour head's too, which another CTA wants at another time (64 requests of up
+    // to 16,000 keys, 8 key heads of 64 columns: 229 us with 128, 299 with 256).
+    const CUtensorMapL2promotion fetch =
+        c->head_dim <= 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
     const struct { CUtensorMap* map; void* base; int64_t slot, head, page; } side[2] = {
         {k, c->k, c->k_slot_stride, c->k_head_stride, c->k_page_stride},
         {v, c->v, c->v_slot_stride, c->v_head_stride, c->v_page_stride}};
     for (const auto& s : side) {
         const cuuint64_t stride[3] = {(cuuint64_t)s.slot * 2, (cuuint64_t)s.head * 2, (cuuint64_t)s.page * 2};
         const CUresult r = enc(s.map, type, 4, s.base, dim, stride, shape, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                               CU_TENSOR_MAP_SWIZZLE_128B, fetch,
                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
         if (r != CUDA_SUCCESS)
             return fail(MARS_ERR_INVALID, "mars_paged_attention: the cache's strides make no tensor map (" +
@@ -146,7 +151,7 @@ extern "C" int mars_paged_attention(mars_kv_ctx* c, const mars_kv_cache* cache, 
     // The short kernel's tiles have 16 rows: with more it would read the keys once for
     // every 16, the chunk kernel once for every 256 but with three launches and tiles
     // of 128 rows (64 ragged requests, 4 query heads a key head: 4 new tokens 202 us
-    // here, 5 there 259; 4 requests of 700 keys: 14 us and 18).
+    // here, 5 there 259; 4 requests of 700 keys on the device: 11 us and 18).
     const bool chunk = (int64_t)std::max(cfg->max_new, 1) * a.group > kShortRows;
     MARS_TRY(kv_attn_memory(c, chunk));
     AttnWork w{};

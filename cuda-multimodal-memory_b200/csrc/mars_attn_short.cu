@@ -52,7 +52,8 @@ constexpr int kRing = 96 * 1024;
 
 // A tile is 32 KB of keys and values: 128 keys of up to 64 columns, 64 of up to
 // 128.  (64 keys of 64 columns, 16 KB, left what a tile costs beside its bytes
-// -- barriers, masks, maxima, rescaling -- in the way: 4.0 TB/s.)
+// -- barriers, masks, maxima, rescaling -- in the way: 4 requests of 700 keys
+// 14.4 us, with 128 keys 11.3.)
 template <int kPanels> struct Layout {
     static constexpr int kTile = 128 / kPanels;                   // keys
     static constexpr int kPer = kTile / kConsumers;               // of a warp: 32 or 16
@@ -545,7 +546,8 @@ int attn_short(const AttnArgs& a, AttnWork w, const mars_kv_cache* cache, int nu
     MARS_TRY(page_maps(cache, w.box, &mk, &mv));
     // Small calls: 128 keys a CTA.  A piece costs 2 to 3 us beside its tiles (its rows'
     // queries, the warps' joining, the output), so fewer and larger shares are slower
-    // (1 request of 100 keys, 12 heads: 7.4 us with 2, 11.0 with 4, 25.5 with 12).
+    // (1 request of 100 keys, 12 heads, in tiles of 64: 7.4 us with 2, 11.0 with 4, 25.5
+    // with 12).
     w.min_share = a.D <= 64 ? 1 : 2;
     if (cache->dtype == MARS_DTYPE_F16)
         return a.D <= 64 ? launch<__half, 1>(a, w, mk, mv, num_sms, st) : launch<__half, 2>(a, w, mk, mv, num_sms, st);
