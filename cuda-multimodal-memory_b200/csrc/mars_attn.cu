@@ -140,11 +140,9 @@ extern "C" int mars_paged_attention(mars_kv_ctx* c, const mars_kv_cache* cache, 
     cudaStream_t st;
     MARS_TRY(kv_begin(c, stream, &st));
     AttnArgs a{};
-    a.q = d_q; a.out = d_out; a.lse = d_lse; a.k = cache->k; a.v = cache->v;
+    a.q = d_q; a.out = d_out; a.lse = d_lse;
     a.cu_new = d_cu_new; a.kv_lens = d_kv_lens; a.tables = d_tables; a.prefix = d_prefix_lens; a.decay = d_decay;
     a.q_tok = q_token_stride; a.q_head = q_head_stride; a.o_tok = out_token_stride; a.o_head = out_head_stride;
-    a.k_page = cache->k_page_stride; a.k_slot = cache->k_slot_stride; a.k_head = cache->k_head_stride;
-    a.v_page = cache->v_page_stride; a.v_slot = cache->v_slot_stride; a.v_head = cache->v_head_stride;
     a.scale = cfg->scale; a.cap = cfg->softcap; a.window = cfg->window;
     a.T = tokens; a.B = B; a.hq = q_heads; a.hkv = cache->kv_heads; a.group = q_heads / cache->kv_heads;
     a.D = cache->head_dim; a.page = cache->page_size; a.num_pages = cache->num_pages; a.pitch = table_pitch;

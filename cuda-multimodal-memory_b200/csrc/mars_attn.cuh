@@ -22,15 +22,12 @@ struct AttnArgs {
     const void* q;                // tokens x q_heads x D
     void* out;
     float* lse;                   // tokens x q_heads, or NULL
-    const void* k;
-    const void* v;
     const int32_t* cu_new;        // B + 1
     const int32_t* kv_lens;       // B
     const int32_t* tables;        // B x pitch
     const int32_t* prefix;        // B, or NULL
     const float* decay;           // q_heads, or NULL
     int64_t q_tok, q_head, o_tok, o_head;
-    int64_t k_page, k_slot, k_head, v_page, v_slot, v_head;
     float scale, cap;             // cap 0: none
     int32_t window;               // 0: none
     int32_t T, B, hq, hkv, group, D, page, num_pages, pitch;
