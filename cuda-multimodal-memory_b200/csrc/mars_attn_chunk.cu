@@ -505,7 +505,10 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
             // keys that all rows of the tile see, besides the prefix
             const int first_pos = k.r.len - k.r.rows + tok0;
             const int all_hi = min(k.r.len, first_pos + 1), all_lo = a.window > 0 ? first_pos + toks - a.window : 0;
-            float m = -INFINITY, l = 0.0f;
+            // A lane without a row has scores of whatever lies there (another request's queries,
+            // an earlier launch's shared memory).  Its maximum is out of reach from the start, so
+            // that it never moves those of the warp's rows.
+            float m = valid ? -INFINITY : INFINITY, l = 0.0f;
 
             for (int j = 0; j < n && ok; ++j) {
                 const int key_tile = key_of(k.u, k.begin + j);
@@ -528,7 +531,9 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
 #pragma unroll
                             for (int i = 0; i < kHalf; i += 2)
                                 far = max3(far, fabsf(__uint_as_float(sr[i])), fabsf(__uint_as_float(sr[i + 1])));
-                            if (__all_sync(0xffffffffu, far * fabsf(in) <= 0.5f && far < 1e18f)) {      // its square is finite
+                            // The score alone says which form of tanh it takes; the vote
+                            // says only whether the warp needs the second one.
+                            if (__all_sync(0xffffffffu, (hi | pre) == 0 || tanh_is_small(far, in))) {
                                 // two scores an instruction
 #pragma unroll
                                 for (int i = 0; i < kHalf; i += 2) {
@@ -537,9 +542,23 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
                                     sr[i + 1] = __float_as_uint(e.y);
                                 }
                             } else {
+                                // In place in TMEM, half the columns at a time: written out over all of
+                                // them, both forms cost the way above 3 % (registers, instruction cache).
+#pragma unroll 1
+                                for (int c = 0; c < 2; ++c) {
+                                    uint32_t x[32];
+                                    tmem_load(tm + c * 32, x);
 #pragma unroll
-                                for (int i = 0; i < kHalf; ++i)
-                                    sr[i] = __float_as_uint(out * tanh_exp(__uint_as_float(sr[i]) * in));
+                                    for (int i = 0; i < 32; i += 2) {
+                                        const float x0 = __uint_as_float(x[i]), x1 = __uint_as_float(x[i + 1]);
+                                        const float2 e = split(tanh_small(pair(x0, x1), small));
+                                        x[i] = __float_as_uint(tanh_is_small(x0, in) ? e.x : out * tanh_exp(x0 * in));
+                                        x[i + 1] = __float_as_uint(tanh_is_small(x1, in) ? e.y : out * tanh_exp(x1 * in));
+                                    }
+                                    tmem_st_32x32b_x32(tm + c * 32, x);
+                                }
+                                tmem_st_wait();
+                                tmem_load(tm, sr);
                             }
                         } else {
 #pragma unroll

@@ -157,6 +157,11 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
     return r;
 }
 
+// Whether s takes the polynomial below (its square has to be finite).
+__device__ __forceinline__ bool tanh_is_small(float s, float in) {
+    return fabsf(s) * fabsf(in) <= 0.5f && fabsf(s) < 1e18f;
+}
+
 // out * tanh(in * s) for |in * s| <= 1/2 as s P(s^2), P a polynomial of degree 5
 // fitted here to the least largest relative error of tanh(x) / x (2^-24.5 in
 // fp32), its coefficients taking the powers of in and out.  No special function:
