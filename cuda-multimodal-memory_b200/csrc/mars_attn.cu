@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <mutex>
 #include <string>
 
@@ -27,6 +28,28 @@ PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
             fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
     });
     return fn;
+}
+
+Cap make_cap(float scale, float softcap) {
+    constexpr float kMost = 3.402823466e38f, kLog2e = 1.4426950408889634f;
+    const float fit[6] = {1.0f, -0.333333283662796f, 0.13332964479923248f, -0.053899191319942474f, 0.021297989413142204f,
+                          -0.006647486239671707f};
+    Cap t{};
+    if (softcap == 0.0f) return t;
+    t.in = std::min(std::max(scale / softcap, -kMost), kMost);      // finite: 0 times it is 0
+    t.out = std::min(softcap * kLog2e, kMost);
+    float power = scale * kLog2e, c = 0.0f;                // in * out, also where those are at the type's ends
+    for (int k = 0; k < 6; ++k) {
+        c = fit[k] * power;
+        uint32_t bits;
+        memcpy(&bits, &c, 4);
+        t.c[k] = (uint64_t)bits << 32 | bits;
+        power *= t.in * t.in;
+    }
+    // s * s is finite up to 1e18.  A cap so small that the powers overflow: its scores are
+    // next to nothing, tanh_exp's error with them.
+    t.most = std::isfinite(c) ? std::min(0.5f / std::fabs(t.in), 1e18f) : -1.0f;
+    return t;
 }
 
 }  // namespace
@@ -143,7 +166,7 @@ extern "C" int mars_paged_attention(mars_kv_ctx* c, const mars_kv_cache* cache, 
     a.q = d_q; a.out = d_out; a.lse = d_lse;
     a.cu_new = d_cu_new; a.kv_lens = d_kv_lens; a.tables = d_tables; a.prefix = d_prefix_lens; a.decay = d_decay;
     a.q_tok = q_token_stride; a.q_head = q_head_stride; a.o_tok = out_token_stride; a.o_head = out_head_stride;
-    a.scale = cfg->scale; a.cap = cfg->softcap; a.window = cfg->window;
+    a.scale = cfg->scale; a.softcap = cfg->softcap; a.cap = make_cap(cfg->scale, cfg->softcap); a.window = cfg->window;
     a.T = tokens; a.B = B; a.hq = q_heads; a.hkv = cache->kv_heads; a.group = q_heads / cache->kv_heads;
     a.D = cache->head_dim; a.page = cache->page_size; a.num_pages = cache->num_pages; a.pitch = table_pitch;
     // The short kernel's tiles have 16 rows: with more it would read the keys once for

@@ -18,6 +18,19 @@
 
 namespace mars {
 
+// A cap: out * tanh(in * s), in units of log 2.  Up to |in * s| = 1/2 as s P(s^2),
+// P a polynomial of degree 5 fitted here to the least largest relative error of
+// tanh(x) / x (2^-24.5 in fp32), its coefficients taking the powers of in and out;
+// beyond it by tanh_exp.  So the error is relative to the score, not to the cap.
+// Which form a score takes follows from the score alone: the same in both kernels,
+// whatever stands beside it.
+// The polynomial has no special function: with two of them for a tanh and one for
+// the softmax, capped scores took three times the exponentials' time.
+struct Cap {
+    float in, out, most;          // most: the largest |s| for the polynomial
+    uint64_t c[6];                // each twice, for two scores an instruction
+};
+
 struct AttnArgs {
     const void* q;                // tokens x q_heads x D
     void* out;
@@ -28,7 +41,8 @@ struct AttnArgs {
     const int32_t* prefix;        // B, or NULL
     const float* decay;           // q_heads, or NULL
     int64_t q_tok, q_head, o_tok, o_head;
-    float scale, cap;             // cap 0: none
+    float scale, softcap;         // softcap 0: none
+    Cap cap;
     int32_t window;               // 0: none
     int32_t T, B, hq, hkv, group, D, page, num_pages, pitch;
 };
@@ -59,11 +73,12 @@ __device__ __forceinline__ void row_range(const AttnArgs& a, const Request& r, i
 
 // tanh x = 1 - 2 / (1 + e^2x): exact to a few units of 2^-24 of 1, so of the
 // cap for the capped score (tanh.approx keeps 2^-11 of the cap, 0.02 at a cap
-// of 50).  Two instructions of the special function unit.
+// of 50).  Two instructions of the special function unit; volatile, because a
+// branch around each where the result is selected took twice the time.
 __device__ __forceinline__ float tanh_exp(float x) {
     float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * 2.8853900817779268f));      // 2 / ln 2
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));                     // 1 / inf = 0
+    asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * 2.8853900817779268f));      // 2 / ln 2
+    asm volatile("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));                     // 1 / inf = 0
     return fmaf(-2.0f, r, 1.0f);
 }
 

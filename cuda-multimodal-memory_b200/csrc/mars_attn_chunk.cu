@@ -490,7 +490,6 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
         const int t = (warp - 4) >> 2, row = tid - 128 - t * 128;
         const uint32_t tm_s = tmem + ((uint32_t)(warp & 3) << 21) + t * 128;      // lanes of this warp
         const uint32_t tm_o = tm_s + 256;
-        const SmallTanh small = kShaped && a.cap > 0.0f ? small_tanh(a.scale / a.cap, a.cap * kLog2e) : SmallTanh{};
         int seen_tiles = 0;                       // the phase of each half's barriers
         for (; more && ok; more = k.next(a, per)) {
             if (t >= k.u.nq) continue;
@@ -525,37 +524,35 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
                     float f = a.scale * kLog2e, top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                     if (kShaped) {
                         // the score in units of log 2 itself
-                        if (a.cap > 0.0f) {
-                            const float in = a.scale / a.cap, out = a.cap * kLog2e;
+                        if (a.softcap > 0.0f) {
                             float far = 0.0f;         // the largest |score| of the row
 #pragma unroll
                             for (int i = 0; i < kHalf; i += 2)
                                 far = max3(far, fabsf(__uint_as_float(sr[i])), fabsf(__uint_as_float(sr[i + 1])));
                             // The score alone says which form of tanh it takes; the vote
                             // says only whether the warp needs the second one.
-                            if (__all_sync(0xffffffffu, (hi | pre) == 0 || tanh_is_small(far, in))) {
-                                // two scores an instruction
+                            if (__all_sync(0xffffffffu, (hi | pre) == 0 || cap_is_small(far, a.cap))) {
 #pragma unroll
                                 for (int i = 0; i < kHalf; i += 2) {
-                                    const float2 e = split(tanh_small(pair(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), small));
+                                    const float2 e = cap_small(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1]), a.cap);
                                     sr[i] = __float_as_uint(e.x);
                                     sr[i + 1] = __float_as_uint(e.y);
                                 }
                             } else {
-                                // In place in TMEM, half the columns at a time: written out over all of
-                                // them, both forms cost the way above 3 % (registers, instruction cache).
+                                // In place in TMEM, 16 columns at a time: written out over all 64 in
+                                // registers, this way took 281 us for 8 capped chunks instead of 216 and
+                                // the one above 187 instead of 178 (32 at a time: 228 and 185).
 #pragma unroll 1
-                                for (int c = 0; c < 2; ++c) {
-                                    uint32_t x[32];
-                                    tmem_load(tm + c * 32, x);
+                                for (int c = 0; c < 4; ++c) {
+                                    uint32_t x[16];
+                                    tmem_load(tm + c * 16, x);
 #pragma unroll
-                                    for (int i = 0; i < 32; i += 2) {
-                                        const float x0 = __uint_as_float(x[i]), x1 = __uint_as_float(x[i + 1]);
-                                        const float2 e = split(tanh_small(pair(x0, x1), small));
-                                        x[i] = __float_as_uint(tanh_is_small(x0, in) ? e.x : out * tanh_exp(x0 * in));
-                                        x[i + 1] = __float_as_uint(tanh_is_small(x1, in) ? e.y : out * tanh_exp(x1 * in));
+                                    for (int i = 0; i < 16; i += 2) {
+                                        const float2 e = cap_any(__uint_as_float(x[i]), __uint_as_float(x[i + 1]), a.cap);
+                                        x[i] = __float_as_uint(e.x);
+                                        x[i + 1] = __float_as_uint(e.y);
                                     }
-                                    tmem_st_32x32b_x32(tm + c * 32, x);
+                                    tmem_st_32x32b_x16(tm + c * 16, x);
                                 }
                                 tmem_st_wait();
                                 tmem_load(tm, sr);
@@ -795,7 +792,7 @@ int attn_chunk(const AttnArgs& a, AttnWork w, const mars_kv_cache* cache, int nu
     MARS_TRY(page_maps(cache, w.box, &mk, &mv));
     MARS_TRY(query_map(a, cache->dtype, kRows / a.group, &mq));
     // scores that a positive factor alone turns into exponents, or not
-    const bool shaped = a.cap > 0.0f || a.decay != nullptr || !(a.scale > 0.0f);
+    const bool shaped = a.softcap > 0.0f || a.decay != nullptr || !(a.scale > 0.0f);
     auto go = [&](auto type, auto panels) {
         using T = decltype(type);
         constexpr int kPanels = decltype(panels)::value;

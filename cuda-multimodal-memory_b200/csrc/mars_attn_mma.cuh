@@ -157,37 +157,21 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
     return r;
 }
 
-// Whether s takes the polynomial below (its square has to be finite).
-__device__ __forceinline__ bool tanh_is_small(float s, float in) {
-    return fabsf(s) * fabsf(in) <= 0.5f && fabsf(s) < 1e18f;
-}
-
-// out * tanh(in * s) for |in * s| <= 1/2 as s P(s^2), P a polynomial of degree 5
-// fitted here to the least largest relative error of tanh(x) / x (2^-24.5 in
-// fp32), its coefficients taking the powers of in and out.  No special function:
-// with two of them for a tanh and one for the softmax, capped scores took three
-// times the exponentials' time.
-struct SmallTanh {
-    float c[6];
-};
-__device__ __forceinline__ SmallTanh small_tanh(float in, float out) {
-    const float fit[6] = {1.0f, -0.333333283662796f, 0.13332964479923248f, -0.053899191319942474f, 0.021297989413142204f,
-                          -0.006647486239671707f};
-    SmallTanh t;
-    float power = in * out;
+// Whether s takes the polynomial.
+__device__ __forceinline__ bool cap_is_small(float s, const Cap& t) { return fabsf(s) <= t.most; }
+// Two scores that both do.
+__device__ __forceinline__ float2 cap_small(float x, float y, const Cap& t) {
+    const uint64_t s = pair(x, y), u = mul2(s, s);
+    uint64_t p = t.c[5];
 #pragma unroll
-    for (int k = 0; k < 6; ++k) {
-        t.c[k] = fit[k] * power;
-        power *= in * in;
-    }
-    return t;
+    for (int k = 4; k >= 0; --k) p = fma2(p, u, t.c[k]);
+    return split(mul2(s, p));
 }
-__device__ __forceinline__ uint64_t tanh_small(uint64_t s, const SmallTanh& t) {
-    const uint64_t u = mul2(s, s);
-    uint64_t p = pair(t.c[5], t.c[5]);
-#pragma unroll
-    for (int k = 4; k >= 0; --k) p = fma2(p, u, pair(t.c[k], t.c[k]));
-    return mul2(s, p);
+// Two scores of any size.
+__device__ __forceinline__ float2 cap_any(float x, float y, const Cap& t) {
+    const float fx = t.out * tanh_exp(x * t.in), fy = t.out * tanh_exp(y * t.in);
+    const float2 e = cap_small(x, y, t);
+    return make_float2(cap_is_small(x, t) ? e.x : fx, cap_is_small(y, t) ? e.y : fy);
 }
 
 // Programmatic dependent launch: the next kernel of the stream may start; wait
@@ -313,6 +297,23 @@ __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) {
           "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
           "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {"
+        "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+        : "memory");
 }
 __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[64]) {
     asm volatile(

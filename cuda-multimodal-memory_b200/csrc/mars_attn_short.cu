@@ -287,12 +287,31 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
                 }
             }
             // in units of log 2
-            if (a.cap > 0.0f) {
-                const float in = a.scale / a.cap, out = a.cap * kLog2e;
+            if (a.softcap > 0.0f) {
+                float far = 0.0f;
 #pragma unroll
                 for (int nb = 0; nb < kBlocks; ++nb)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[nb][e] = out * tanh_exp(s[nb][e] * in);
+                    for (int e = 0; e < 4; e += 2) far = max3(far, fabsf(s[nb][e]), fabsf(s[nb][e + 1]));
+                if (__all_sync(0xffffffffu, cap_is_small(far, a.cap))) {
+#pragma unroll
+                    for (int nb = 0; nb < kBlocks; ++nb)
+#pragma unroll
+                        for (int e = 0; e < 4; e += 2) {
+                            const float2 v = cap_small(s[nb][e], s[nb][e + 1], a.cap);
+                            s[nb][e] = v.x;
+                            s[nb][e + 1] = v.y;
+                        }
+                } else {
+#pragma unroll
+                    for (int nb = 0; nb < kBlocks; ++nb)
+#pragma unroll
+                        for (int e = 0; e < 4; e += 2) {
+                            const float2 v = cap_any(s[nb][e], s[nb][e + 1], a.cap);
+                            s[nb][e] = v.x;
+                            s[nb][e + 1] = v.y;
+                        }
+                }
             } else {
                 const float f = a.scale * kLog2e;
 #pragma unroll
