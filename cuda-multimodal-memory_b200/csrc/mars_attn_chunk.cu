@@ -647,7 +647,7 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
             }
             const bool whole = k.begin == 0 && k.end == k.u.tiles;
             const int slot = 2 * blockIdx.x + (k.begin == 0);
-            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             T* out = reinterpret_cast<T*>(a.out) + (int64_t)(k.r.first + tok) * a.o_tok + (int64_t)head * a.o_head;
             float* part = w.chunk_o + (int64_t)slot * kPartCols * 2 * kRows + t * kRows + row;
             // TMEM loads are for the whole warp: lanes without a row take part, and all
@@ -683,7 +683,7 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
                 }
             }
             if (valid && whole && a.lse != nullptr)
-                a.lse[(int64_t)(k.r.first + tok) * a.hq + head] = l > 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+                a.lse[(int64_t)(k.r.first + tok) * a.hq + head] = log_sum(m, l);
             if (valid && !whole) w.chunk_ml[slot * 2 * kRows + t * kRows + row] = make_float2(m, l);
         }
     }
@@ -725,9 +725,9 @@ __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const AttnArgs a, 
     for (int n = 0; n < parts; ++n) top = fmaxf(top, w.chunk_ml[slot(n) * 2 * kRows + row].x);
     for (int n = 0; n < parts; ++n) {
         const float2 ml = w.chunk_ml[slot(n) * 2 * kRows + row];
-        if (ml.x != -INFINITY) sum += ml.y * exp2f_fast(ml.x - top);
+        sum += scaled_sum(ml.x, ml.y, top);
     }
-    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     const int head = s.h * a.group + in % a.group;
     T* out = reinterpret_cast<T*>(a.out) + (int64_t)(r.first + tok) * a.o_tok + (int64_t)head * a.o_head;
     for (int d = warp * 8; d < a.D; d += 64) {
@@ -745,7 +745,7 @@ __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const AttnArgs a, 
                        pack2<T>(v[4] * inv, v[5] * inv), pack2<T>(v[6] * inv, v[7] * inv));
     }
     if (warp == 0 && a.lse != nullptr)
-        a.lse[(int64_t)(r.first + tok) * a.hq + head] = sum > 0.0f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+        a.lse[(int64_t)(r.first + tok) * a.hq + head] = log_sum(top, sum);
 }
 
 // Launches a kernel whose set-up may overlap the end of the one before it in the

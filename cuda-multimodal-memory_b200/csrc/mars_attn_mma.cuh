@@ -123,6 +123,16 @@ __device__ __forceinline__ float exp2f_fast(float x) {
     return y;
 }
 
+// A part's sum, at maximum m, on the scale of top.  Without a maximum it is 0, or
+// NaN: maxima pass over scores that are NaN, sums keep them.
+__device__ __forceinline__ float scaled_sum(float m, float sum, float top) {
+    return m == -INFINITY ? sum : sum * exp2f_fast(m - top);
+}
+// lse of a row (maximum in units of log 2): -inf only where nothing was seen.
+__device__ __forceinline__ float log_sum(float top, float sum) {
+    return sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+}
+
 // Two fp32 values in one register pair, and the packed arithmetic on them (one
 // instruction for both).
 __device__ __forceinline__ uint64_t pair(float x, float y) {

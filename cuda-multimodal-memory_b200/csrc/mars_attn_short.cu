@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
         for (int x = 0; x < kConsumers; ++x) top = fmaxf(top, s_m[x][row]);
 #pragma unroll
         for (int x = 0; x < kConsumers; ++x)
-            if (s_m[x][row] != -INFINITY) sum += s_l[x][row] * exp2f_fast(s_m[x][row] - top);
+            sum += scaled_sum(s_m[x][row], s_l[x][row], top);
 
         const long long at = x1 - cur.left - begin;           // the unit's place in the sequence
         const int c0 = (int)(at / share), parts = (int)((at + c - 1) / share) - c0 + 1;
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
 #pragma unroll 4
                 for (int p = col0; p < parts; p += 8) {
                     const float2 ml = __ldcg(&w.part_ml[(2 * (c0 + p) + (p == 0)) * kRows + r_]);
-                    if (ml.x != -INFINITY) sum += ml.y * exp2f_fast(ml.x - top);
+                    sum += scaled_sum(ml.x, ml.y, top);
                 }
 #pragma unroll
                 for (int off = 1; off < 8; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
@@ -495,10 +495,10 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
         if (write) {
             if (col0 == 0) {
                 s_top[row] = top;
-                s_inv[row] = sum > 0.0f ? 1.0f / sum : 0.0f;
+                s_inv[row] = sum == 0.0f ? 0.0f : 1.0f / sum;
                 if (row < valid && a.lse != nullptr) {
                     const int tok = r.first + u.row0 + row / a.group, head = head0 + row % a.group;
-                    a.lse[(int64_t)tok * a.hq + head] = sum > 0.0f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+                    a.lse[(int64_t)tok * a.hq + head] = log_sum(top, sum);
                 }
             }
             bar_sync(1, 32 * kConsumers);

@@ -708,8 +708,8 @@ int mars_rope_append(const mars_rope_table* table, const mars_kv_cache* cache, c
  * softmax form, with the distance in tokens as the age.  out = the softmax's
  * mean of the values; lse (may be NULL) = log of the sum of exp(score), by
  * which two parts of an attention are joined.  A row that sees nothing gets
- * out = 0 and lse = -inf.  Query head h reads key head h / (q_heads /
- * kv_heads).  d_decay and d_prefix_lens may be NULL (none).
+ * out = 0 and lse = -inf, one that sees a score that is NaN gets NaN in both.
+ * Query head h reads key head h / (q_heads / kv_heads).  d_decay and d_prefix_lens may be NULL (none).
  *
  * q, out: tokens x q_heads x head_dim of the cache's dtype; lse: tokens x
  * q_heads fp32.  Tokens from d_cu_new[B] on are left alone.  max_new is the
