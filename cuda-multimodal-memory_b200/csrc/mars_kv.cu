@@ -78,28 +78,34 @@ int kv_begin(mars_kv_ctx* c, void* stream, cudaStream_t* st) {
     if (*static_cast<volatile int*>(c->h_err) != 0) {
         // the kernel that gave up has ended all the same; start the next one clean
         MARS_CUDA_TRY(cudaEventSynchronize(c->used));
-        MARS_CUDA_TRY(cudaMemsetAsync(c->d_err, 0, sizeof(int), c->last));
-        MARS_CUDA_TRY(cudaEventRecord(c->used, c->last));
+        MARS_CUDA_TRY(cudaMemsetAsync(c->d_err, 0, sizeof(int), c->stream));
+        MARS_CUDA_TRY(cudaEventRecord(c->used, c->stream));
+        c->last_id = ~0ull;                        // the next call waits, whatever its stream
+        c->any = true;
         const int code = *c->h_err;
         *c->h_err = 0;
         return fail(MARS_ERR_TIMEOUT, "an earlier call's bounded wait " + std::to_string(code) +
                                           " gave up: its results are not valid");
     }
     *st = stream != nullptr ? static_cast<cudaStream_t>(stream) : c->stream;
-    if (c->any && *st != c->last) {
-        cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-        MARS_CUDA_TRY(cudaStreamIsCapturing(*st, &cap));
-        if (cap == cudaStreamCaptureStatusNone) MARS_CUDA_TRY(cudaStreamWaitEvent(*st, c->used, 0));
-    }
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    MARS_CUDA_TRY(cudaStreamIsCapturing(*st, &cap));
+    c->captured = cap != cudaStreamCaptureStatusNone;
+    if (c->captured) return MARS_OK;               // a replay's order is its launcher's
+    // The id tells streams apart, their handles do not: a destroyed stream's may be a new
+    // one's, and cudaStreamPerThread is another stream in every thread.  (Waiting on the same
+    // stream too would be as right, and 0.3 us of host time a call.)
+    unsigned long long id = 0;
+    MARS_CUDA_TRY(cudaStreamGetId(*st, &id));
+    if (c->any && id != c->last_id) MARS_CUDA_TRY(cudaStreamWaitEvent(*st, c->used, 0));
+    c->now_id = id;
     return MARS_OK;
 }
 
 int kv_end(mars_kv_ctx* c, cudaStream_t st) {
-    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    MARS_CUDA_TRY(cudaStreamIsCapturing(st, &cap));
-    if (cap != cudaStreamCaptureStatusNone) return MARS_OK;   // a replay's order is its launcher's
+    if (c->captured) return MARS_OK;
     MARS_CUDA_TRY(cudaEventRecord(c->used, st));
-    c->last = st;
+    c->last_id = c->now_id;
     c->any = true;
     return MARS_OK;
 }

@@ -35,9 +35,11 @@ struct mars_kv_ctx {
 
     // The working memory above holds one call at a time.  `used` is recorded
     // after every call outside a capture; a call on another stream waits for it.
-    cudaStream_t last = nullptr;
     cudaEvent_t used = nullptr;
     bool any = false;
+    unsigned long long last_id = 0;     // that call's stream (cudaStreamGetId)
+    unsigned long long now_id = 0;      // the call under way: its stream,
+    bool captured = false;              // and whether it is part of a capture
 };
 
 namespace mars {

@@ -596,7 +596,9 @@ int mars_scan_topk_noalloc(const float* d_embeddings, int32_t row_pitch,
  * layer.  All pointers are device pointers, all calls asynchronous on
  * `stream` (NULL: the context's stream).  A context holds the working memory
  * of one call at a time: calls on several streams are ordered one after the
- * other (inside a stream capture, by the order of the launches of the graph). */
+ * other, whatever becomes of the streams.  A captured call is ordered by its
+ * graph alone: its replays and the context's other calls are the caller's to
+ * order.  Host threads use a context one at a time. */
 #define MARS_KV_MAX_REQUESTS 8192
 typedef struct mars_kv_ctx mars_kv_ctx;
 
