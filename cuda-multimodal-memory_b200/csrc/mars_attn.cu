@@ -176,8 +176,11 @@ extern "C" int mars_paged_attention(mars_kv_ctx* c, const mars_kv_cache* cache, 
     const bool chunk = (int64_t)std::max(cfg->max_new, 1) * a.group > kShortRows;
     MARS_TRY(kv_attn_memory(c, chunk));
     AttnWork w{};
-    w.part_o = c->d_part_o; w.part_ml = c->d_part_ml; w.tickets = c->d_tickets + kKvTickets; w.err = c->d_err;
+    w.part_o = c->d_part_o; w.part_ml = c->d_part_ml; w.tickets = c->d_tickets + kKvTickets;
     w.host_err = c->h_err; w.chunk_o = c->d_chunk_o; w.chunk_ml = c->d_chunk_ml; w.starts = c->d_starts;
+    w.failed = c->d_failed;
+    w.wait_ns = c->wait_ns; w.stall = c->stall ? 0 : -1;
+    c->stall = false;
     const int done = chunk ? attn_chunk(a, w, cache, c->num_sms, st) : attn_short(a, w, cache, c->num_sms, st);
     const int end = kv_end(c, st);                 // also after an error: some launches may be under way
     return done != MARS_OK ? done : end;

@@ -129,7 +129,8 @@ __device__ long long plan_scan(long long v, long long* total) {
 }
 
 // starts[i]: where CTA i's share begins; starts[ctas]: the end.
-__global__ void __launch_bounds__(kPlanThreads) attn_chunk_plan_kernel(const AttnArgs a, ChunkStart* starts, int ctas) {
+__global__ void __launch_bounds__(kPlanThreads) attn_chunk_plan_kernel(const AttnArgs a, ChunkStart* starts, int* failed,
+                                                                       int ctas) {
     launch_dependents();                          // the main kernel sets itself up meanwhile
     extern __shared__ int s_units[];              // B: units (of one head) before request b
     const int per = kRows / a.group;
@@ -177,6 +178,7 @@ __global__ void __launch_bounds__(kPlanThreads) attn_chunk_plan_kernel(const Att
     }
     for (long long i = threadIdx.x; i <= ctas; i += kPlanThreads)
         if (i == ctas || i * share >= total) starts[i] = ChunkStart{a.B, 0, 0, 0};
+    for (int i = threadIdx.x; i < ctas; i += kPlanThreads) failed[i] = 0;
 }
 
 // ---- the kernel -------------------------------------------------------------
@@ -198,9 +200,9 @@ struct Walk {
         count[0] = u.nq == 2 ? max(0, min(u.tiles0 - begin, n)) : n;
         count[1] = u.nq == 2 ? n : 0;
     }
-    __device__ __forceinline__ bool start(const AttnArgs& a, const ChunkStart* starts, int per) {
-        cur = starts[blockIdx.x];
-        stop = starts[blockIdx.x + 1];
+    __device__ __forceinline__ bool start(const AttnArgs& a, const ChunkStart* starts, int cta, int per) {
+        cur = starts[cta];
+        stop = starts[cta + 1];
         if (done()) return false;
         r = load_request(a, cur.b);
         set(a, per);
@@ -253,11 +255,14 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
     __shared__ uint64_t s_qfull, s_qempty, s_full[L::kSlots], s_ready[L::kSlots], s_empty[L::kSlots];
     __shared__ uint64_t s_sfull[2][2], s_pfull[2][2], s_odone[2][2], s_drain[2];      // [row tile][half]
     __shared__ uint32_t s_tmem;
+    __shared__ int s_err;
+    const WaitLimit limit{&s_err, w.wait_ns};
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int per = kRows / a.group;              // tokens of a row tile
     const int ksteps = (a.D + 15) / 16;
 
     if (tid == 0) {
+        s_err = 0;
         mbar_init(&s_qfull, 1);
         mbar_init(&s_qempty, 2);
         for (int i = 0; i < L::kSlots; ++i) {
@@ -291,16 +296,17 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
     bool ok = true;
     if (warp < 4) {
         Walk k;
-        bool more = k.start(a, starts, per);
+        bool more = k.start(a, starts, blockIdx.x, per);
         if (warp == 0) {
             // ---- loads -------------------------------------------------------------
             const int boxes = kTile / w.box;
             const bool on = lane < boxes * kPanels;
             const int panel = lane / boxes, at = (lane % boxes) * w.box;
             int slot_no = 0, q_no = 0;
+            if (blockIdx.x == w.stall) more = false;
             for (; more && ok; more = k.next(a, per)) {
                 if (k.begin == k.end) continue;       // nothing visible: no tile, no query
-                if (q_no > 0 && !warp_wait(&s_qempty, (q_no - 1) & 1, w.err, 1)) { ok = false; break; }
+                if (q_no > 0 && !warp_wait<true>(&s_qempty, (q_no - 1) & 1, limit, 1)) { ok = false; break; }
                 ++q_no;
                 if (lane == 0) mbar_arrive_expect_tx(&s_qfull, k.u.nq * kPanels * per * a.group * 128);
                 __syncwarp();
@@ -321,7 +327,7 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
 #pragma unroll
                     for (int side = 0; side < 2; ++side, ++slot_no) {
                         const int slot = slot_no % L::kSlots, phase = (slot_no / L::kSlots) & 1;
-                        if (slot_no >= L::kSlots && !warp_wait(&s_empty[slot], phase ^ 1, w.err, 2)) {
+                        if (slot_no >= L::kSlots && !warp_wait<true>(&s_empty[slot], phase ^ 1, limit, 2)) {
                             ok = false;
                             break;
                         }
@@ -335,8 +341,8 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
             }
             // no copy may be in flight when the CTA ends
             for (int i = max(0, slot_no - L::kSlots); i < slot_no; ++i)
-                drain_wait(&s_full[i % L::kSlots], (i / L::kSlots) & 1, w.err, 3);
-            if (q_no > 0) drain_wait(&s_qfull, (q_no - 1) & 1, w.err, 3);
+                drain_wait<true>(&s_full[i % L::kSlots], (i / L::kSlots) & 1, limit, 3);
+            if (q_no > 0) drain_wait<true>(&s_qfull, (q_no - 1) & 1, limit, 3);
         } else if (warp != 2) {
             // ---- products of row tile t ----------------------------------------------
             // The warp stays together: every lane walks and waits, an elected one issues.
@@ -357,7 +363,7 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
             int q_no = 0, steps[2] = {0, 0};          // queries freed; weights multiplied, by half
             int s_done = 0;                           // scores made of second halves
             auto wait = [&](uint64_t* bar, int phase, int code) {
-                ok = ok && warp_wait(bar, phase & 1, w.err, code);
+                ok = ok && warp_wait<true>(bar, phase & 1, limit, code);
                 return ok;
             };
             // S = Q K^T of 64 keys.  It overwrites P: products with different accumulators
@@ -447,10 +453,10 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
             // No product may be in flight when TMEM is freed, and no commit's arrival
             // when the CTA's shared memory is: the last of each barrier is awaited.
             if (elect_one()) mma_commit(&s_drain[t]);
-            drain_wait(&s_drain[t], 0, w.err, 10);
-            if (steps[0] > 0) drain_wait(&s_odone[t][0], (steps[0] - 1) & 1, w.err, 10);
-            if (steps[1] > 0) drain_wait(&s_odone[t][1], (steps[1] - 1) & 1, w.err, 10);
-            if (s_done > 0) drain_wait(&s_sfull[t][1], (s_done - 1) & 1, w.err, 10);
+            drain_wait<true>(&s_drain[t], 0, limit, 10);
+            if (steps[0] > 0) drain_wait<true>(&s_odone[t][0], (steps[0] - 1) & 1, limit, 10);
+            if (steps[1] > 0) drain_wait<true>(&s_odone[t][1], (steps[1] - 1) & 1, limit, 10);
+            if (s_done > 0) drain_wait<true>(&s_sfull[t][1], (s_done - 1) & 1, limit, 10);
             __syncwarp();
         } else {
             // ---- values that no row sees ----------------------------------------------
@@ -459,11 +465,11 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
                 for (int t = k.begin; t < k.end; ++t) {
                     // The keys too, in the ring's order: loads land in any order, and a
                     // parity tells only neighbouring uses of a slot apart.
-                    ok = ok && warp_wait(&s_full[ring.slot], ring.phase, w.err, 10);
+                    ok = ok && warp_wait<true>(&s_full[ring.slot], ring.phase, limit, 10);
                     if (!ok) break;
                     ring.step();
                     const int slot = ring.slot;
-                    ok = ok && warp_wait(&s_full[slot], ring.phase, w.err, 10);
+                    ok = ok && warp_wait<true>(&s_full[slot], ring.phase, limit, 10);
                     if (!ok) break;
                     ring.step();
                     const int key0 = key_of(k.u, t);
@@ -486,7 +492,7 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
     } else {
         // ---- softmax: warpgroup t, a thread for each row ------------------------------
         Walk k;
-        bool more = k.start(a, starts, per);
+        bool more = k.start(a, starts, blockIdx.x, per);
         const int t = (warp - 4) >> 2, row = tid - 128 - t * 128;
         const uint32_t tm_s = tmem + ((uint32_t)(warp & 3) << 21) + t * 128;      // lanes of this warp
         const uint32_t tm_o = tm_s + 256;
@@ -513,7 +519,7 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
                 const int key_tile = key_of(k.u, k.begin + j);
 #pragma unroll 1
                 for (int h = 0; h < 2; ++h) {
-                    ok = ok && warp_wait(&s_sfull[t][h], seen_tiles & 1, w.err, 11);
+                    ok = ok && warp_wait<true>(&s_sfull[t][h], seen_tiles & 1, limit, 11);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t tm = tm_s + h * kHalf;
@@ -599,7 +605,7 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
                         const float keep = to == -INFINITY ? 1.0f : exp2f_fast(m - to);
                         if (j + h > 0) {
                             // once the products of the steps before are in O
-                            ok = ok && warp_wait(&s_odone[t][h ^ 1], (seen_tiles + h + 1) & 1, w.err, 14);
+                            ok = ok && warp_wait<true>(&s_odone[t][h ^ 1], (seen_tiles + h + 1) & 1, limit, 14);
                             if (!ok) break;
                             tc_fence_after();
                             for (int c = 0; c * 32 < a.D; ++c) {
@@ -641,7 +647,7 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
             // ---- the piece's end -------------------------------------------------
             // the product of the last step, which those before it are part of
             if (n > 0) {
-                ok = ok && warp_wait(&s_odone[t][1], (seen_tiles - 1) & 1, w.err, 12);
+                ok = ok && warp_wait<true>(&s_odone[t][1], (seen_tiles - 1) & 1, limit, 12);
                 if (!ok) break;
                 tc_fence_after();
             }
@@ -687,7 +693,7 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
             if (valid && !whole) w.chunk_ml[slot * 2 * kRows + t * kRows + row] = make_float2(m, l);
         }
     }
-    if (!ok && lane == 0) *w.host_err = *(volatile int*)w.err;
+    if (lane == 0) report_wait(limit, w.host_err, w.failed + blockIdx.x);
     tc_fence_before();
     __syncthreads();
     if (warp == 1) {
@@ -698,13 +704,39 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
 
 // ---- cut units ----------------------------------------------------------------
 
+// Whole units of a CTA whose wait gave up: NaN in each of its rows.
+template <typename T>
+__device__ void mark_units(const AttnArgs& a, const ChunkStart* starts, int cta) {
+    const int per = kRows / a.group, t = threadIdx.x / kRows, row = threadIdx.x % kRows;
+    Walk k;
+    for (bool more = k.start(a, starts, cta, per); more; more = k.next(a, per)) {
+        const int toks = min(per, k.u.rows - t * per);
+        if (k.begin != 0 || k.end != k.u.tiles || row >= toks * a.group) continue;
+        const int64_t tok = k.r.first + k.u.row0 + t * per + row / a.group;
+        const int head = k.cur.h * a.group + row % a.group;
+        T* out = reinterpret_cast<T*>(a.out) + tok * a.o_tok + (int64_t)head * a.o_head;
+        const uint32_t none = pack2<T>(NAN, NAN);
+        for (int d = 0; d < a.D; d += 8) *reinterpret_cast<uint4*>(out + d) = make_uint4(none, none, none, none);
+        if (a.lse != nullptr) a.lse[tok * a.hq + head] = NAN;
+    }
+}
+
+constexpr int kJoinBlocks = 2 * kRows / 32;
+
 // Block (i, group of 32 rows): if share i begins inside a unit and is the first
 // to, joins the unit's parts, in their order: share i-1's end, then i, i+1, ...
+// Rows that a CTA left without a result, because a wait of it gave up, get NaN
+// (whole units by the blocks of a row group more).
 template <typename T>
 __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts,
                                                               int ctas) {
     wait_primary();
     const int i = blockIdx.x + 1;
+    if (blockIdx.y == kJoinBlocks) {
+        if (w.failed[i] != 0) mark_units<T>(a, starts, i);
+        if (i == 1 && w.failed[0] != 0) mark_units<T>(a, starts, 0);
+        return;
+    }
     const ChunkStart s = starts[i], p = starts[i - 1];
     if (s.b >= a.B || s.tile == 0) return;
     if (p.b == s.b && p.qt == s.qt && p.h == s.h && p.tile > 0) return;      // cut before
@@ -725,7 +757,7 @@ __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const AttnArgs a, 
     for (int n = 0; n < parts; ++n) top = fmaxf(top, w.chunk_ml[slot(n) * 2 * kRows + row].x);
     for (int n = 0; n < parts; ++n) {
         const float2 ml = w.chunk_ml[slot(n) * 2 * kRows + row];
-        sum += scaled_sum(ml.x, ml.y, top);
+        sum += w.failed[i - 1 + n] != 0 ? NAN : scaled_sum(ml.x, ml.y, top);
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     const int head = s.h * a.group + in % a.group;
@@ -772,12 +804,12 @@ int launch(const AttnArgs& a, const AttnWork& w, const CUtensorMap& mq, const CU
     using L = Layout<kPanels>;
     static std::atomic<uint64_t> done{0};
     MARS_TRY(allow_smem(reinterpret_cast<const void*>(attn_chunk_kernel<T, kPanels, kFull, kShaped>), L::kSmem, done));
-    attn_chunk_plan_kernel<<<1, kPlanThreads, a.B * sizeof(int), st>>>(a, w.starts, ctas);
+    attn_chunk_plan_kernel<<<1, kPlanThreads, a.B * sizeof(int), st>>>(a, w.starts, w.failed, ctas);
     MARS_CUDA_TRY(cudaGetLastError());
     MARS_TRY(launch_after(attn_chunk_kernel<T, kPanels, kFull, kShaped>, dim3(ctas), kThreads, L::kSmem, st, a, w,
                           (const ChunkStart*)w.starts, mq, mk, mv));
     if (ctas > 1)
-        MARS_TRY(launch_after(attn_chunk_join_kernel<T>, dim3(ctas - 1, 2 * kRows / 32), 256, 0, st, a, w,
+        MARS_TRY(launch_after(attn_chunk_join_kernel<T>, dim3(ctas - 1, kJoinBlocks + 1), 256, 0, st, a, w,
                               (const ChunkStart*)w.starts, ctas));
     return MARS_OK;
 }

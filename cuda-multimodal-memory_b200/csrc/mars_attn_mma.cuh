@@ -33,8 +33,10 @@ struct AttnWork {
     float* chunk_o;               // chunk kernel: slots x kPartCols x 256 rows
     float2* chunk_ml;             // slots x 256 rows
     ChunkStart* starts;           // one for each CTA and the end
-    int* err;                     // device word: a bounded wait gave up
-    int* host_err;                // the same, where the host sees it
+    int* failed;                  // one for each CTA: a wait of it gave up
+    int* host_err;                // host memory: code of a bounded wait that gave up
+    uint64_t wait_ns;             // their limit
+    int stall;                    // test hook: this CTA loads nothing, so its waits run out (-1: none)
     int box;                      // keys of one TMA box: divides a page and a tile
     int min_share;                // tiles a CTA takes at least
 };
@@ -49,17 +51,21 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const void* tmap, ui
 }
 
 // Bounded waits of the attention kernels, for all lanes of a warp: false after
-// two seconds (a step of these pipelines takes microseconds), with `code` in
-// the error word, which ends the other waits too.  drain: keeps waiting for
-// copies or products in flight when others have given up.
-constexpr uint64_t kWaitNs = 2000000000ull;
+// `limit` (two seconds, where a step of these pipelines takes microseconds), with
+// `code` in the CTA's error word, which ends its other waits too.  No CTA waits
+// for another, so the word is the CTA's own, in shared memory: nothing of a wait
+// that gave up is left for other CTAs, calls or replays to meet.  drain: keeps
+// waiting for copies or products in flight when others have given up.
+struct WaitLimit {
+    int* err;                     // shared
+    uint64_t ns;
+};
 __device__ __forceinline__ uint64_t now_ns() {
     uint64_t t;
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
     return t;
 }
-__device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, int* err, int code, bool drain) {
-    if (sm100::mbar_try_wait(bar, parity)) return true;
+__device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity, int* err, uint64_t limit_ns, int code, bool drain) {
     // Kept small (unrolled, the polls of twenty waits were most of a 148 KB
     // kernel, and its path through them missed the instruction cache).
     uint64_t begin = 0;
@@ -69,17 +75,39 @@ __device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, int
         if ((i & 63u) == 0) {
             const uint64_t now = now_ns();
             if (begin == 0) begin = now;
-            if (now - begin > kWaitNs || (!drain && *((volatile int*)err) != 0)) break;
+            if (now - begin > limit_ns || (!drain && *((volatile int*)err) != 0)) break;
         }
     }
     atomicCAS(err, 0, code);
     return false;
 }
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
-    return __all_sync(0xffffffffu, bounded_wait(bar, parity, err, code, false));
+inline __device__ __noinline__ bool wait_on_far(uint64_t* bar, uint32_t parity, int* err, uint64_t limit_ns, int code, bool drain) {
+    return wait_on(bar, parity, err, limit_ns, code, drain);
 }
-__device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
-    bounded_wait(bar, parity, err, code, true);
+// kFar: what follows a first poll that fails stands out of line, once for all waits.
+// The chunk kernel has twenty of them (8 capped chunks 188 us written out, 174 out of
+// line; prompts 830 and 783), the short kernel two (64 ragged requests 197 us written
+// out, 211 out of line).
+template <bool kFar>
+__device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, const WaitLimit& limit, int code, bool drain) {
+    if (sm100::mbar_try_wait(bar, parity)) return true;
+    return kFar ? wait_on_far(bar, parity, limit.err, limit.ns, code, drain)
+                : wait_on(bar, parity, limit.err, limit.ns, code, drain);
+}
+template <bool kFar = false>
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const WaitLimit& limit, int code) {
+    return __all_sync(0xffffffffu, bounded_wait<kFar>(bar, parity, limit, code, false));
+}
+template <bool kFar = false>
+__device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity, const WaitLimit& limit, int code) {
+    bounded_wait<kFar>(bar, parity, limit, code, true);
+}
+// Tells the host, and `failed` if there is one, of a wait of this CTA that gave up.
+__device__ __forceinline__ void report_wait(const WaitLimit& limit, int* host_err, int* failed = nullptr) {
+    const int code = *((volatile int*)limit.err);
+    if (code == 0) return;
+    *host_err = code;
+    if (failed != nullptr) *failed = code;
 }
 
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }

@@ -104,11 +104,13 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
     __shared__ float s_m[kConsumers][kRows], s_l[kConsumers][kRows], s_top[kRows], s_inv[kRows];
     __shared__ long long s_sum[kThreads / 32 + 1];
     __shared__ Found s_found;
-    __shared__ int s_last;
+    __shared__ int s_last, s_err;
+    const WaitLimit limit{&s_err, w.wait_ns};
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int per = kRows / a.group;              // tokens of a row tile
 
     if (tid == 0) {
+        s_err = 0;
         for (int i = 0; i < L::kStages; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&s_empty[i], kConsumers);
@@ -171,7 +173,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
         const CUtensorMap* map = is_v ? &map_v : &map_k;
         const int dst = ((is_v ? kPanels : 0) + panel) * kTile * 128 + at * 128;
         int issued = 0;
-        bool ok = true;
+        bool ok = blockIdx.x != w.stall;
         while (ok && cur.left > 0) {
             const Unit u = make_unit<kTile>(a, r, cur.qt, per);
             const int c = max(1, u.tiles), end = (int)min((long long)c, cur.tile + cur.left);
@@ -189,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
             for (int t = cur.tile; t < min(end, u.tiles); ++t) {
                 const int stage = issued % L::kStages, phase = (issued / L::kStages) & 1;
                 if (issued >= L::kStages &&
-                    !warp_wait(&s_empty[stage], phase ^ 1, w.err, 1)) { ok = false; break; }
+                    !warp_wait(&s_empty[stage], phase ^ 1, limit, 1)) { ok = false; break; }
                 if (lane == 0) mbar_arrive_expect_tx(&s_full[stage], L::kStage);
                 __syncwarp();
                 const int key = (t < u.n1 ? t : u.s2 + t - u.n1) * kTile + at;
@@ -210,8 +212,8 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
         }
         // no copy may be in flight when the CTA ends
         for (int i = max(0, issued - L::kStages); i < issued; ++i)
-            drain_wait(&s_full[i % L::kStages], (i / L::kStages) & 1, w.err, 2);
-        if (!ok && lane == 0) *w.host_err = *(volatile int*)w.err;
+            drain_wait(&s_full[i % L::kStages], (i / L::kStages) & 1, limit, 2);
+        if (lane == 0) report_wait(limit, w.host_err);
         return;
     }
 
@@ -262,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
         for (int t = begin; t < min(end, u.tiles); ++t, ++used) {
             const int stage = used % L::kStages;
             // a wait that gave up: the unit's barriers are still taken, so that no warp is left at one
-            ok = ok && warp_wait(&s_full[stage], (used / L::kStages) & 1, w.err, 3);
+            ok = ok && warp_wait(&s_full[stage], (used / L::kStages) & 1, limit, 3);
             if (!ok) continue;
             const int key0 = (t < u.n1 ? t : u.s2 + t - u.n1) * kTile + warp * L::kPer;
             const uint32_t sk = smem_u32(ring + stage * L::kStage) + warp * L::kPer * 128;
@@ -406,6 +408,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
         }
 
         // ---- the unit's part of this share: join the four warps ---------------
+        if (!ok) l[0] = l[1] = NAN;                // a wait gave up: the rows say so
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
@@ -542,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
             }
         }
     }
-    if (!ok && lane == 0) *w.host_err = *(volatile int*)w.err;
+    if (lane == 0) report_wait(limit, w.host_err);
 }
 
 template <typename T, int kPanels>

@@ -69,28 +69,30 @@ int kv_attn_memory(mars_kv_ctx* c, bool chunk) {
         const size_t rows = 256, slots = 2 * sms;
         if (c->d_chunk_o == nullptr) MARS_CUDA_TRY(cudaMalloc(&c->d_chunk_o, slots * rows * kPartCols * sizeof(float)));
         if (c->d_chunk_ml == nullptr) MARS_CUDA_TRY(cudaMalloc(&c->d_chunk_ml, slots * rows * sizeof(float2)));
-        MARS_CUDA_TRY(cudaMalloc(&c->d_starts, (sms + 1) * sizeof(ChunkStart)));
+        MARS_CUDA_TRY(cudaMalloc(&c->d_starts, (sms + 1) * sizeof(ChunkStart) + sms * sizeof(int)));
+        c->d_failed = reinterpret_cast<int*>(c->d_starts + sms + 1);
     }
     return MARS_OK;
 }
 
+int kv_report(mars_kv_ctx* c) {
+    const int code = *static_cast<volatile int*>(c->h_err);
+    if (code == 0) return MARS_OK;
+    *static_cast<volatile int*>(c->h_err) = 0;
+    return fail(MARS_ERR_TIMEOUT, "a bounded wait (" + std::to_string(code) +
+                                      ") of an earlier call gave up: its results are not valid");
+}
+
 int kv_begin(mars_kv_ctx* c, void* stream, cudaStream_t* st) {
-    if (*static_cast<volatile int*>(c->h_err) != 0) {
-        // the kernel that gave up has ended all the same; start the next one clean
-        MARS_CUDA_TRY(cudaEventSynchronize(c->used));
-        MARS_CUDA_TRY(cudaMemsetAsync(c->d_err, 0, sizeof(int), c->stream));
-        MARS_CUDA_TRY(cudaEventRecord(c->used, c->stream));
-        c->last_id = ~0ull;                        // the next call waits, whatever its stream
-        c->any = true;
-        const int code = *c->h_err;
-        *c->h_err = 0;
-        return fail(MARS_ERR_TIMEOUT, "an earlier call's bounded wait " + std::to_string(code) +
-                                          " gave up: its results are not valid");
-    }
     *st = stream != nullptr ? static_cast<cudaStream_t>(stream) : c->stream;
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
     MARS_CUDA_TRY(cudaStreamIsCapturing(*st, &cap));
     c->captured = cap != cudaStreamCaptureStatusNone;
+    if (*static_cast<volatile int*>(c->h_err) != 0) {
+        // All of the call's CTAs have reported once it has ended.
+        if (!c->captured && c->any) MARS_CUDA_TRY(cudaEventSynchronize(c->used));
+        return kv_report(c);
+    }
     if (c->captured) return MARS_OK;               // a replay's order is its launcher's
     // The id tells streams apart, their handles do not: a destroyed stream's may be a new
     // one's, and cudaStreamPerThread is another stream in every thread.  (Waiting on the same
@@ -358,12 +360,12 @@ extern "C" int mars_kv_ctx_create(int32_t device, int32_t max_requests, mars_kv_
     c->device = device;
     c->max_requests = max_requests;
     c->num_sms = sms;
+    c->wait_ns = kWaitNs;
     auto build = [&]() -> int {
         MARS_CUDA_TRY(cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking));
         MARS_CUDA_TRY(cudaEventCreateWithFlags(&c->used, cudaEventDisableTiming));
-        const size_t words = kKvTickets + 2 * (size_t)sms + 1;
+        const size_t words = kKvTickets + 2 * (size_t)sms;
         MARS_CUDA_TRY(cudaMalloc(&c->d_tickets, words * sizeof(unsigned int)));
-        c->d_err = reinterpret_cast<int*>(c->d_tickets + kKvTickets + 2 * (size_t)sms);
         MARS_TRY(host_word(&c->h_err));
         *c->h_err = 0;
         MARS_CUDA_TRY(cudaMemsetAsync(c->d_tickets, 0, words * sizeof(unsigned int), c->stream));
@@ -396,6 +398,20 @@ extern "C" int mars_kv_ctx_destroy(mars_kv_ctx* c) {
     if (c->used != nullptr) cudaEventDestroy(c->used);
     if (c->stream != nullptr) cudaStreamDestroy(c->stream);
     delete c;
+    return MARS_OK;
+}
+
+extern "C" int mars_kv_ctx_status(mars_kv_ctx* c) {
+    if (c == nullptr) return fail(MARS_ERR_INVALID, "mars_kv_ctx_status: NULL context");
+    MarsDeviceGuard g(c->device);
+    if (c->any) MARS_CUDA_TRY(cudaEventSynchronize(c->used));
+    return kv_report(c);
+}
+
+extern "C" int mars_kv_ctx_debug_wait(mars_kv_ctx* c, uint64_t limit_ns, int32_t stall) {
+    if (c == nullptr) return fail(MARS_ERR_INVALID, "mars_kv_ctx_debug_wait: NULL context");
+    c->wait_ns = limit_ns == 0 ? kWaitNs : limit_ns;
+    c->stall = stall != 0;
     return MARS_OK;
 }
 

@@ -23,15 +23,16 @@ struct mars_kv_ctx {
     unsigned int* d_tickets = nullptr;
 
     // Attention: parts of units that several CTAs share (mars_attn_short.cu),
-    // and the word that a bounded wait which gave up sets, on the device for
-    // the kernel's other warps and in mapped host memory for the next call.
+    // and the word, in mapped host memory, that a bounded wait which gave up sets.
     float* d_part_o = nullptr;
     float2* d_part_ml = nullptr;
     float* d_chunk_o = nullptr;         // the same for mars_attn_chunk.cu
     float2* d_chunk_ml = nullptr;
     mars::ChunkStart* d_starts = nullptr;
-    int* d_err = nullptr;
+    int* d_failed = nullptr;            // after the starts, in the same allocation
     int* h_err = nullptr;
+    uint64_t wait_ns = 0;               // the waits' limit
+    bool stall = false;                 // test hook: the next attention call's first CTA loads nothing
 
     // The working memory above holds one call at a time.  `used` is recorded
     // after every call outside a capture; a call on another stream waits for it.
@@ -50,6 +51,10 @@ constexpr int kKvTickets = 2;
 
 // The attention kernels' parts (5 or 39 MB), made by the first call of each kind.
 int kv_attn_memory(mars_kv_ctx* c, bool chunk);
+constexpr uint64_t kWaitNs = 2000000000ull;
+
+// MARS_ERR_TIMEOUT, once, if a wait has given up since the last report.
+int kv_report(mars_kv_ctx* c);
 // The stream of a call on `c`, ordered after the context's previous call.
 int kv_begin(mars_kv_ctx* c, void* stream, cudaStream_t* st);
 // Marks the end of the call's work on `st`.

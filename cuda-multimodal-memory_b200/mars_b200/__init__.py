@@ -170,6 +170,8 @@ _SIGS = {
 _SIGS.update({
     "mars_kv_ctx_create": [_I32, _I32, C.POINTER(_VP)],
     "mars_kv_ctx_destroy": [_VP],
+    "mars_kv_ctx_status": [_VP],
+    "mars_kv_ctx_debug_wait": [_VP, C.c_uint64, _I32],
     "mars_kv_release": [_VP, _I32, _VP, _VP, _VP, _I32, _I32, _VP, _I32, _VP, _VP, _VP, _VP, _VP],
     "mars_kv_plan": [_VP, _I32, _VP, _VP, _VP, _I32, _I32, _VP, _I32, _VP, _I32, _VP, _VP, _VP, _VP, _VP, _VP,
                      _VP],

@@ -186,6 +186,16 @@ class KvContext:
         if t.get_device() != self.device:
             raise ValueError(f"the context works on device {self.device}, a tensor is on {t.device}")
 
+    def status(self):
+        """Waits for the context's last call; raises MarsError (MARS_ERR_TIMEOUT) if a bounded wait of an attention call
+        has given up since the last report.  Rows that it left without a result are NaN in out and lse."""
+        _check(lib().mars_kv_ctx_status(self.handle))
+
+    def debug_wait(self, limit_ns: int = 0, stall: bool = False) -> None:
+        """Test hook: the attention kernels' waits give up after limit_ns (0: the default); stall: the next attention
+        call's first CTA loads nothing, so that its waits run out."""
+        _check(lib().mars_kv_ctx_debug_wait(self.handle, limit_ns, int(stall)))
+
     def release(self, kv_lens, finished, tables, free_pages, free_count, *, page_size, status=None, stream=None):
         """Push the pages of the requests with finished != 0 onto the free stack; returns the new
         (kv_lens, free_count).  A failure (status, one int32, if given) leaves everything as it was."""

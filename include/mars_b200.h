@@ -608,6 +608,18 @@ typedef struct mars_kv_ctx mars_kv_ctx;
 int mars_kv_ctx_create(int32_t device, int32_t max_requests, mars_kv_ctx** out);
 /* Waits for the context's last call.  NULL is accepted. */
 int mars_kv_ctx_destroy(mars_kv_ctx* ctx);
+/* Waits for the context's last call.  MARS_ERR_TIMEOUT if a bounded device wait
+ * of an attention call has given up since the last report (of captured calls:
+ * of the replays that have ended).  Rows that it left without a result are NaN
+ * in out and lse; what the caller computed from them is as invalid, for the
+ * report comes after the calls that it had queued by then.  Those find nothing
+ * of it: a later call with valid inputs has valid results. */
+int mars_kv_ctx_status(mars_kv_ctx* ctx);
+/* Test hook for those waits (as mars_batch_ctx_debug_wait).  limit_ns bounds
+ * each (0: the default, two seconds).  stall != 0: the first CTA of the next
+ * attention call loads nothing, so that its waits cannot end and give up after
+ * limit_ns; the call after it runs normally. */
+int mars_kv_ctx_debug_wait(mars_kv_ctx* ctx, uint64_t limit_ns, int32_t stall);
 
 /* Bits of *d_status of mars_kv_release and mars_kv_plan (0: done).  A call
  * that sets one leaves tables, stack, lengths and counts as they were, and
@@ -723,8 +735,8 @@ int mars_rope_append(const mars_rope_table* table, const mars_kv_cache* cache, c
  * influence, non-finite values included; of the keys below the length, the
  * values must be finite.  A table entry outside [0, num_pages) reads as zero
  * keys and values.
- * A bounded device wait that gave up is returned as MARS_ERR_TIMEOUT by the
- * context's next call; the call it happened in has no valid results.
+ * A bounded device wait that gave up is returned as MARS_ERR_TIMEOUT by
+ * mars_kv_ctx_status, or by the context's next call, which then does nothing.
  * Limits: head_dim a multiple of 8 up to 128, page_size a multiple of 8, at
  * most 128 query heads a key head, at most MARS_ATTN_MAX_KEYS keys a request;
  * all rows on 16-byte boundaries. */
