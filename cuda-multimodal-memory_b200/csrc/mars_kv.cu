@@ -401,6 +401,8 @@ extern "C" int mars_kv_ctx_destroy(mars_kv_ctx* c) {
     return MARS_OK;
 }
 
+extern "C" void* mars_kv_ctx_stream(const mars_kv_ctx* c) { return c != nullptr ? c->stream : nullptr; }
+
 extern "C" int mars_kv_ctx_status(mars_kv_ctx* c) {
     if (c == nullptr) return fail(MARS_ERR_INVALID, "mars_kv_ctx_status: NULL context");
     MarsDeviceGuard g(c->device);

@@ -182,7 +182,8 @@ _SIGS.update({
                              _I64, _I64, _VP, _VP],
 })
 _RESTYPE = {"mars_last_error": C.c_char_p, "mars_status_string": C.c_char_p,
-            "mars_abi_version": C.c_int, "mars_query_ctx_stream": C.c_void_p}
+            "mars_abi_version": C.c_int, "mars_query_ctx_stream": C.c_void_p,
+            "mars_kv_ctx_stream": C.c_void_p}
 
 _lib = None
 
@@ -203,6 +204,7 @@ def lib() -> C.CDLL:
             getattr(L, name).restype = rt
         L.mars_status_string.argtypes = [C.c_int]
         L.mars_query_ctx_stream.argtypes = [_VP]
+        L.mars_kv_ctx_stream.argtypes = [_VP]
         _lib = L
     return _lib
 

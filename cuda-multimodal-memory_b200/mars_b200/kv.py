@@ -12,7 +12,10 @@ rope is the rotation by itself, for programs that train; its gradient is
 rope(..., inverse=True) of the output's gradient.
 
 All arguments are torch CUDA tensors; calls run on torch's current stream
-unless one is given, and return without waiting.
+unless one is given (its handle, an integer), and return without waiting.  On a
+given stream the caller orders the call after what makes its inputs, and keeps
+them (record_stream) while it runs, as with torch's own operators; what the call
+allocates itself belongs to that stream, and may be dropped at any time.
 """
 from __future__ import annotations
 
@@ -51,6 +54,23 @@ def _stream(stream, t):
     if stream is not None:
         return stream
     return _raw_stream(t.get_device()) or _STREAM_LEGACY
+
+
+def _empty(stream, t, shape, dtype):
+    """An output of a call on the given stream (None: torch's current one on t's device).  The memory belongs to that
+    stream, so that it goes to nobody else before the call has run; and the current stream, where the caller goes on, is
+    recorded, so that a later call on the given one does not get it too early."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=t.device)
+    handle = getattr(stream, "value", stream) or 0
+    on = torch.cuda.default_stream(t.device) if handle in (0, _STREAM_LEGACY) else \
+        torch.cuda.ExternalStream(handle, device=t.device)
+    here = torch.cuda.current_stream(t.device)
+    with torch.cuda.stream(on):
+        made = torch.empty(shape, dtype=dtype, device=t.device)
+    if here != on:
+        made.record_stream(here)
+    return made
 
 
 def _on_device_of(t, call, args):
@@ -133,9 +153,9 @@ def _table(tokens, positions, freq, axis, interleaved):
     return _Table(freq.data_ptr(), axis.data_ptr(), 2 * freq.shape[0], axes, int(interleaved), 0)
 
 
-def _out(out, x):
+def _out(out, x, stream):
     if out is None:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        return _empty(stream, x, x.shape, x.dtype)
     if out.shape != x.shape:
         raise ValueError("out must have the input's shape")
     return out
@@ -150,7 +170,7 @@ def rope(x, positions, freq, axis, *, interleaved=False, inverse=False, out=None
         raise ValueError("x must be fp32, fp16 or bf16")
     n, heads, dim = x.shape
     table = _table(n, positions, freq, axis, interleaved)
-    out = _out(out, x)
+    out = _out(out, x, stream)
     _on_device_of(x, lib().mars_rope, (C.byref(table), dtype, *xp, *_heads("out", out, x), n, heads, dim,
                                        positions.data_ptr(), int(inverse), _stream(stream, x)))
     return out
@@ -167,7 +187,7 @@ def rope_append(q, k, v, positions, freq, axis, cache, slots, *, interleaved=Fal
         raise ValueError("q, k and v must have the cache's type, device, heads and columns")
     table = _table(n, positions, freq, axis, interleaved)
     slots = _ints("slots", slots, n)
-    out = _out(out, q)
+    out = _out(out, q, stream)
     _on_device_of(q, lib().mars_rope_append, (C.byref(table), cache._ref, *qp, *kp, *vp, *_heads("out", out, q), n, heads,
                                               positions.data_ptr(), slots, _stream(stream, q)))
     return out
@@ -181,6 +201,10 @@ class KvContext:
         _check(lib().mars_kv_ctx_create(device, max_requests, C.byref(h)))
         self.handle = h
         self.device = device
+
+    def _given(self, stream):
+        """The handle of a given stream (0: the context's own)."""
+        return getattr(stream, "value", stream) or lib().mars_kv_ctx_stream(self.handle)
 
     def _here(self, t):
         if t.get_device() != self.device:
@@ -201,7 +225,11 @@ class KvContext:
         (kv_lens, free_count).  A failure (status, one int32, if given) leaves everything as it was."""
         self._here(kv_lens)
         B = kv_lens.shape[0]
-        lens_out, count_out = torch.empty_like(kv_lens), torch.empty_like(free_count)
+        if stream is None:
+            lens_out, count_out = torch.empty_like(kv_lens), torch.empty_like(free_count)
+        else:
+            stream = self._given(stream)
+            lens_out, count_out = (_empty(stream, x, x.shape, torch.int32) for x in (kv_lens, free_count))
         _check(lib().mars_kv_release(
             self.handle, B, _ints("kv_lens", kv_lens), _ints("finished", finished, B),
             _ints("tables", tables, B, 2), tables.shape[1], page_size, _ints("free_pages", free_pages),
@@ -213,10 +241,11 @@ class KvContext:
         """Pages (into tables, in place), slots and positions for new_lens more tokens of each request."""
         self._here(kv_lens)
         B = kv_lens.shape[0]
+        if stream is not None:
+            stream = self._given(stream)
         # one allocation for all that comes back
-        lens_out, cu_new, slots, positions, count_out, status = torch.empty(
-            2 * (B + max_tokens) + 3, dtype=torch.int32, device=kv_lens.device).split(
-                (B, B + 1, max_tokens, max_tokens, 1, 1))
+        lens_out, cu_new, slots, positions, count_out, status = _empty(
+            stream, kv_lens, 2 * (B + max_tokens) + 3, torch.int32).split((B, B + 1, max_tokens, max_tokens, 1, 1))
         _check(lib().mars_kv_plan(
             self.handle, B, _ints("kv_lens", kv_lens), _ints("new_lens", new_lens, B), _ints("tables", tables, B, 2),
             tables.shape[1], page_size, _ints("free_pages", free_pages), free_pages.shape[0],
@@ -244,8 +273,10 @@ class KvContext:
                     decay.shape != (heads,):
                 raise ValueError("decay must be a contiguous float32 CUDA tensor of q_heads entries")
             decay = decay.data_ptr()
-        out = _out(out, q)
-        lse = torch.empty((n, heads), dtype=torch.float32, device=q.device) if return_lse else None
+        if stream is not None:
+            stream = self._given(stream)
+        out = _out(out, q, stream)
+        lse = _empty(stream, q, (n, heads), torch.float32) if return_lse else None
         cfg = _Config(dim ** -0.5 if scale is None else scale, softcap, window, n if max_new is None else max_new)
         _check(lib().mars_paged_attention(
             self.handle, cache._ref, *qp, n, heads, B, _ints("cu_new", cu_new, B + 1), _ints("kv_lens", kv_lens),

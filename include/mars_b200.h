@@ -608,6 +608,8 @@ typedef struct mars_kv_ctx mars_kv_ctx;
 int mars_kv_ctx_create(int32_t device, int32_t max_requests, mars_kv_ctx** out);
 /* Waits for the context's last call.  NULL is accepted. */
 int mars_kv_ctx_destroy(mars_kv_ctx* ctx);
+/* The context's own stream, on which calls with stream == NULL run. */
+void* mars_kv_ctx_stream(const mars_kv_ctx* ctx);
 /* Waits for the context's last call.  MARS_ERR_TIMEOUT if a bounded device wait
  * of an attention call has given up since the last report (of captured calls:
  * of the replays that have ended).  Rows that it left without a result are NaN
