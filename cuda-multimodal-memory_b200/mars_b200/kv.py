@@ -82,11 +82,21 @@ def _on_device_of(t, call, args):
             _check(call(*args))
 
 
-def _ints(name, t, n=None, dims=1):
-    """The address of a contiguous int32 CUDA tensor of n entries (n None: any)."""
+def _ints(name, t, device, n=None, dims=1):
+    """The address of a contiguous int32 tensor of n entries (n None: any) on the CUDA device of that number."""
     shape = t.shape
-    if t.dtype is not torch.int32 or not t.is_cuda or len(shape) != dims or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 CUDA tensor of {dims} dimension(s)")
+    if t.dtype is not torch.int32 or t.get_device() != device or len(shape) != dims or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {dims} dimension(s) on cuda:{device}")
+    if n is not None and shape[0] != n:
+        raise ValueError(f"{name} must have {n} entries, has {shape[0]}")
+    return t.data_ptr()
+
+
+def _floats(name, t, device, n=None):
+    """The same of a float32 tensor of one dimension."""
+    shape = t.shape
+    if t.dtype is not torch.float32 or t.get_device() != device or len(shape) != 1 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous float32 tensor of 1 dimension on cuda:{device}")
     if n is not None and shape[0] != n:
         raise ValueError(f"{name} must have {n} entries, has {shape[0]}")
     return t.data_ptr()
@@ -142,15 +152,14 @@ def _heads(name, x, like=None):
     return x.data_ptr(), strides[0], strides[1]
 
 
-def _table(tokens, positions, freq, axis, interleaved):
-    _ints("positions", positions, tokens, positions.dim())
+def _table(tokens, positions, freq, axis, interleaved, device):
+    _ints("positions", positions, device, tokens, positions.dim())
     if positions.dim() not in (1, 2):
         raise ValueError("positions must be [tokens] or [tokens, axes]")
-    if freq.dtype is not torch.float32 or not freq.is_cuda or not freq.is_contiguous() or freq.dim() != 1:
-        raise ValueError("freq must be a contiguous float32 CUDA tensor of 1 dimension")
-    _ints("axis", axis, freq.shape[0])
+    pairs = freq.shape[0] if freq.dim() == 1 else None
+    freq = _floats("freq", freq, device)
     axes = 1 if positions.dim() == 1 else positions.shape[1]
-    return _Table(freq.data_ptr(), axis.data_ptr(), 2 * freq.shape[0], axes, int(interleaved), 0)
+    return _Table(freq, _ints("axis", axis, device, pairs), 2 * pairs, axes, int(interleaved), 0)
 
 
 def _out(out, x, stream):
@@ -169,7 +178,7 @@ def rope(x, positions, freq, axis, *, interleaved=False, inverse=False, out=None
     if dtype is None:
         raise ValueError("x must be fp32, fp16 or bf16")
     n, heads, dim = x.shape
-    table = _table(n, positions, freq, axis, interleaved)
+    table = _table(n, positions, freq, axis, interleaved, x.get_device())
     out = _out(out, x, stream)
     _on_device_of(x, lib().mars_rope, (C.byref(table), dtype, *xp, *_heads("out", out, x), n, heads, dim,
                                        positions.data_ptr(), int(inverse), _stream(stream, x)))
@@ -185,8 +194,8 @@ def rope_append(q, k, v, positions, freq, axis, cache, slots, *, interleaved=Fal
     if q.dtype is not cache.k.dtype or q.device != cache.k.device or dim != c.head_dim or \
             k.shape[1:] != (c.kv_heads, dim) or v.shape != k.shape:
         raise ValueError("q, k and v must have the cache's type, device, heads and columns")
-    table = _table(n, positions, freq, axis, interleaved)
-    slots = _ints("slots", slots, n)
+    table = _table(n, positions, freq, axis, interleaved, q.get_device())
+    slots = _ints("slots", slots, q.get_device(), n)
     out = _out(out, q, stream)
     _on_device_of(q, lib().mars_rope_append, (C.byref(table), cache._ref, *qp, *kp, *vp, *_heads("out", out, q), n, heads,
                                               positions.data_ptr(), slots, _stream(stream, q)))
@@ -206,10 +215,6 @@ class KvContext:
         """The handle of a given stream (0: the context's own)."""
         return getattr(stream, "value", stream) or lib().mars_kv_ctx_stream(self.handle)
 
-    def _here(self, t):
-        if t.get_device() != self.device:
-            raise ValueError(f"the context works on device {self.device}, a tensor is on {t.device}")
-
     def status(self):
         """Waits for the context's last call; raises MarsError (MARS_ERR_TIMEOUT) if a bounded wait of an attention call
         has given up since the last report.  Rows that it left without a result are NaN in out and lse."""
@@ -223,33 +228,33 @@ class KvContext:
     def release(self, kv_lens, finished, tables, free_pages, free_count, *, page_size, status=None, stream=None):
         """Push the pages of the requests with finished != 0 onto the free stack; returns the new
         (kv_lens, free_count).  A failure (status, one int32, if given) leaves everything as it was."""
-        self._here(kv_lens)
-        B = kv_lens.shape[0]
+        d, B = self.device, kv_lens.shape[0]
+        pointers = (_ints("kv_lens", kv_lens, d), _ints("finished", finished, d, B), _ints("tables", tables, d, B, 2),
+                    tables.shape[1], page_size, _ints("free_pages", free_pages, d), free_pages.shape[0],
+                    _ints("free_count", free_count, d, 1))
+        status = None if status is None else _ints("status", status, d, 1)
         if stream is None:
             lens_out, count_out = torch.empty_like(kv_lens), torch.empty_like(free_count)
         else:
             stream = self._given(stream)
             lens_out, count_out = (_empty(stream, x, x.shape, torch.int32) for x in (kv_lens, free_count))
         _check(lib().mars_kv_release(
-            self.handle, B, _ints("kv_lens", kv_lens), _ints("finished", finished, B),
-            _ints("tables", tables, B, 2), tables.shape[1], page_size, _ints("free_pages", free_pages),
-            free_pages.shape[0], _ints("free_count", free_count, 1), lens_out.data_ptr(), count_out.data_ptr(),
-            None if status is None else _ints("status", status, 1), _stream(stream, kv_lens)))
+            self.handle, B, *pointers, lens_out.data_ptr(), count_out.data_ptr(), status, _stream(stream, kv_lens)))
         return lens_out, count_out
 
     def plan(self, kv_lens, new_lens, tables, free_pages, free_count, *, page_size, max_tokens, stream=None) -> KvPlan:
         """Pages (into tables, in place), slots and positions for new_lens more tokens of each request."""
-        self._here(kv_lens)
-        B = kv_lens.shape[0]
+        d, B = self.device, kv_lens.shape[0]
+        pointers = (_ints("kv_lens", kv_lens, d), _ints("new_lens", new_lens, d, B), _ints("tables", tables, d, B, 2),
+                    tables.shape[1], page_size, _ints("free_pages", free_pages, d), free_pages.shape[0],
+                    _ints("free_count", free_count, d, 1))
         if stream is not None:
             stream = self._given(stream)
         # one allocation for all that comes back
         lens_out, cu_new, slots, positions, count_out, status = _empty(
             stream, kv_lens, 2 * (B + max_tokens) + 3, torch.int32).split((B, B + 1, max_tokens, max_tokens, 1, 1))
         _check(lib().mars_kv_plan(
-            self.handle, B, _ints("kv_lens", kv_lens), _ints("new_lens", new_lens, B), _ints("tables", tables, B, 2),
-            tables.shape[1], page_size, _ints("free_pages", free_pages), free_pages.shape[0],
-            _ints("free_count", free_count, 1), max_tokens, lens_out.data_ptr(), count_out.data_ptr(),
+            self.handle, B, *pointers, max_tokens, lens_out.data_ptr(), count_out.data_ptr(),
             cu_new.data_ptr(), slots.data_ptr(), positions.data_ptr(), status.data_ptr(), _stream(stream, kv_lens)))
         return KvPlan(lens_out, cu_new, slots, positions, count_out, status)
 
@@ -266,22 +271,22 @@ class KvContext:
         n, heads, dim = q.shape
         if q.dtype is not cache.k.dtype or q.device != cache.k.device or dim != cache._c.head_dim:
             raise ValueError("q must have the cache's type, device and columns")
-        self._here(q)
-        B = kv_lens.shape[0]
+        d, B = self.device, kv_lens.shape[0]
+        if q.get_device() != d:
+            raise ValueError(f"the context works on cuda:{d}, q and the cache are on {q.device}")
         if decay is not None:
-            if decay.dtype is not torch.float32 or not decay.is_cuda or not decay.is_contiguous() or \
-                    decay.shape != (heads,):
-                raise ValueError("decay must be a contiguous float32 CUDA tensor of q_heads entries")
-            decay = decay.data_ptr()
+            decay = _floats("decay", decay, d, heads)
+        pointers = (_ints("cu_new", cu_new, d, B + 1), _ints("kv_lens", kv_lens, d), _ints("tables", tables, d, B, 2),
+                    tables.shape[1])
+        if prefix_lens is not None:
+            prefix_lens = _ints("prefix_lens", prefix_lens, d, B)
         if stream is not None:
             stream = self._given(stream)
         out = _out(out, q, stream)
         lse = _empty(stream, q, (n, heads), torch.float32) if return_lse else None
         cfg = _Config(dim ** -0.5 if scale is None else scale, softcap, window, n if max_new is None else max_new)
         _check(lib().mars_paged_attention(
-            self.handle, cache._ref, *qp, n, heads, B, _ints("cu_new", cu_new, B + 1), _ints("kv_lens", kv_lens),
-            _ints("tables", tables, B, 2), tables.shape[1], C.byref(cfg), decay,
-            None if prefix_lens is None else _ints("prefix_lens", prefix_lens, B), *_heads("out", out, q),
+            self.handle, cache._ref, *qp, n, heads, B, *pointers, C.byref(cfg), decay, prefix_lens, *_heads("out", out, q),
             None if lse is None else lse.data_ptr(), _stream(stream, q)))
         return (out, lse) if return_lse else out
 
