@@ -8,8 +8,9 @@ A step of a program that answers with retrieved memories:
         q = rope_append(q, k, v, positions, freq, axis, cache, plan.slots)
         out = ctx.attention(q, cache, tables, plan.kv_lens, plan.cu_new, max_new=1)
 
-rope is the rotation by itself, for programs that train; its gradient is
-rope(..., inverse=True) of the output's gradient.
+rope is the rotation by itself, for programs that train: autograd records it,
+and its gradient is rope(..., inverse=True) of the output's gradient.  The calls
+on a cache are for answering and record no gradient.
 
 All arguments are torch CUDA tensors; calls run on torch's current stream
 unless one is given (its handle, an integer), and return without waiting.  On a
@@ -170,9 +171,31 @@ def _out(out, x, stream):
     return out
 
 
+class _Rope(torch.autograd.Function):
+    """rope on an x that requires a gradient: the rotation is orthogonal, so dx is dy turned the other way."""
+
+    @staticmethod
+    def forward(ctx, x, positions, freq, axis, interleaved, inverse, stream):
+        ctx.save_for_backward(positions, freq, axis)
+        ctx.how = interleaved, inverse
+        return rope(x, positions, freq, axis, interleaved=interleaved, inverse=inverse, stream=stream)
+
+    @staticmethod
+    def backward(ctx, dy):
+        interleaved, inverse = ctx.how
+        if dy.stride(2) != 1:
+            dy = dy.contiguous()                   # an expanded gradient (of a sum) has strides of 0
+        return rope(dy, *ctx.saved_tensors, interleaved=interleaved, inverse=not inverse), None, None, None, None, None, None
+
+
 def rope(x, positions, freq, axis, *, interleaved=False, inverse=False, out=None, stream=None):
     """Rotary positions of x [tokens, heads, head_dim] (fp32, fp16 or bf16): pair i turns by positions[:, axis[i]]
-    * freq[i].  positions: int32 [tokens, axes].  inverse: turns back, the gradient of the forward rotation."""
+    * freq[i].  positions: int32 [tokens, axes].  inverse: turns back, the gradient of the forward rotation.  x has a
+    gradient (its backward pass runs on autograd's stream, also where stream is given), freq has none."""
+    if x.requires_grad and torch.is_grad_enabled():
+        if out is not None:
+            raise ValueError("rope into out records no gradient: leave out away, or detach x")
+        return _Rope.apply(x, positions, freq, axis, interleaved, inverse, stream)
     xp = _heads("x", x)
     dtype = _DTYPES.get(x.dtype)
     if dtype is None:
@@ -186,7 +209,7 @@ def rope(x, positions, freq, axis, *, interleaved=False, inverse=False, out=None
 
 
 def rope_append(q, k, v, positions, freq, axis, cache, slots, *, interleaved=False, out=None, stream=None):
-    """q rotated (returned, or into out, which may be q), k rotated and v copied into the cache's slots.
+    """q rotated (returned, or into out, which may be q), k rotated and v copied into the cache's slots.  No gradient.
     q: [tokens, q_heads, head_dim], k and v: [tokens, kv_heads, head_dim], all of the cache's type."""
     qp, kp, vp = _heads("q", q), _heads("k", k, q), _heads("v", v, q)
     n, heads, dim = q.shape
@@ -264,7 +287,10 @@ class KvContext:
         cu_new[b] to cu_new[b+1], already in the cache), over the pages of tables [B, pages].  kv_lens counts the
         new tokens.  A row at position i sees key j when j < prefix_lens[b], or j <= i and (window 0 or i - j <
         window); scores are scale * q.k (scale None: head_dim ** -0.5), capped by softcap * tanh(. / softcap), minus
-        decay[head] * max(0, i - j).  max_new: the most new tokens of one request, if known (it chooses the kernel).
+        decay[head] * max(0, i - j).  No gradient.
+        max_new: the most new tokens of one request.  It chooses the kernel, not the answer: up to 16 rows (max_new times
+        the query heads of a key head) the one for single tokens.  Without it the call has to count on one request's having
+        all tokens, and takes the one for chunks as soon as it has more than a few: give it to every step of single tokens.
         Returns out (q's shape and type), with return_lse also the fp32 [tokens, q_heads] log of the scores'
         exponentials' sum."""
         qp = _heads("q", q)
