@@ -31,6 +31,7 @@ _raw_stream = torch._C._cuda_getCurrentRawStream      # torch.cuda.current_strea
 _current_device = torch._C._cuda_getDevice
 
 KV_MAX_REQUESTS = 8192   # MARS_KV_MAX_REQUESTS
+_INT32_MAX = 2 ** 31 - 1
 
 # bits of KvPlan.status
 KV_BAD_LENGTH = 1
@@ -310,7 +311,9 @@ class KvContext:
             stream = self._given(stream)
         out = _out(out, q, stream)
         lse = _empty(stream, q, (n, heads), torch.float32) if return_lse else None
-        cfg = _Config(dim ** -0.5 if scale is None else scale, softcap, window, n if max_new is None else max_new)
+        # a window or bound beyond 32 bits is none (a C field would keep its low bits)
+        cfg = _Config(dim ** -0.5 if scale is None else scale, softcap, min(window, _INT32_MAX),
+                      min(n if max_new is None else max_new, _INT32_MAX))
         _check(lib().mars_paged_attention(
             self.handle, cache._ref, *qp, n, heads, B, *pointers, C.byref(cfg), decay, prefix_lens, *_heads("out", out, q),
             None if lse is None else lse.data_ptr(), _stream(stream, q)))
