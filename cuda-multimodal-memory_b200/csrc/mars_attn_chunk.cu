@@ -696,6 +696,8 @@ attn_chunk_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts, 
     if (lane == 0) report_wait(limit, w.host_err, w.failed + blockIdx.x);
     tc_fence_before();
     __syncthreads();
+    if (*(volatile int*)&s_err != 0)              // this CTA's parts of cut units have no result
+        for (int i = tid; i < 4 * kRows; i += kThreads) w.chunk_ml[2 * blockIdx.x * 2 * kRows + i] = make_float2(0.0f, NAN);
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
@@ -725,8 +727,9 @@ constexpr int kJoinBlocks = 2 * kRows / 32;
 
 // Block (i, group of 32 rows): if share i begins inside a unit and is the first
 // to, joins the unit's parts, in their order: share i-1's end, then i, i+1, ...
-// Rows that a CTA left without a result, because a wait of it gave up, get NaN
-// (whole units by the blocks of a row group more).
+// Rows that a CTA left without a result, because a wait of it gave up, get NaN:
+// in cut units by their parts' sums, in whole ones here, by the blocks of a row
+// group more (neither costs the kernels' loops anything).
 template <typename T>
 __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const AttnArgs a, const AttnWork w, const ChunkStart* starts,
                                                               int ctas) {
@@ -757,7 +760,7 @@ __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const AttnArgs a, 
     for (int n = 0; n < parts; ++n) top = fmaxf(top, w.chunk_ml[slot(n) * 2 * kRows + row].x);
     for (int n = 0; n < parts; ++n) {
         const float2 ml = w.chunk_ml[slot(n) * 2 * kRows + row];
-        sum += w.failed[i - 1 + n] != 0 ? NAN : scaled_sum(ml.x, ml.y, top);
+        sum += scaled_sum(ml.x, ml.y, top);
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     const int head = s.h * a.group + in % a.group;
