@@ -52,10 +52,10 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const void* tmap, ui
 
 // Bounded waits of the attention kernels, for all lanes of a warp: false after
 // `limit` (two seconds, where a step of these pipelines takes microseconds), with
-// `code` in the CTA's error word, which ends its other waits too.  No CTA waits
-// for another, so the word is the CTA's own, in shared memory: nothing of a wait
-// that gave up is left for other CTAs, calls or replays to meet.  drain: keeps
-// waiting for copies or products in flight when others have given up.
+// `code` in the CTA's error word.  No CTA waits for another, so the word is the
+// CTA's own, in shared memory: nothing of a wait that gave up is left for other
+// CTAs, calls or replays to meet.  drain: a wait for copies or products in flight,
+// which goes on when others have given up.
 struct WaitLimit {
     int* err;                     // shared
     uint64_t ns;
@@ -87,12 +87,14 @@ inline __device__ __noinline__ bool wait_on_far(uint64_t* bar, uint32_t parity, 
 // kFar: what follows a first poll that fails stands out of line, once for all waits.
 // The chunk kernel has twenty of them (8 capped chunks 188 us written out, 174 out of
 // line; prompts 830 and 783), the short kernel two (64 ragged requests 197 us written
-// out, 211 out of line).
+// out, 211 out of line).  The short kernel's also do not look at the error word: its
+// warps wait for the same loads, so their limits run out together (204.0 us with the
+// look, 203.2 without).
 template <bool kFar>
 __device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, const WaitLimit& limit, int code, bool drain) {
     if (sm100::mbar_try_wait(bar, parity)) return true;
     return kFar ? wait_on_far(bar, parity, limit.err, limit.ns, code, drain)
-                : wait_on(bar, parity, limit.err, limit.ns, code, drain);
+                : wait_on(bar, parity, limit.err, limit.ns, code, true);
 }
 template <bool kFar = false>
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const WaitLimit& limit, int code) {

@@ -408,7 +408,6 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
         }
 
         // ---- the unit's part of this share: join the four warps ---------------
-        if (!ok) l[0] = l[1] = NAN;                // a wait gave up: the rows say so
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
@@ -453,6 +452,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const AttnArgs 
 #pragma unroll
         for (int x = 0; x < kConsumers; ++x)
             sum += scaled_sum(s_m[x][row], s_l[x][row], top);
+        if (*(volatile int*)&s_err != 0) sum = NAN;             // a wait gave up: the rows say so
 
         const long long at = x1 - cur.left - begin;           // the unit's place in the sequence
         const int c0 = (int)(at / share), parts = (int)((at + c - 1) / share) - c0 + 1;
