@@ -171,8 +171,8 @@ extern "C" int mars_paged_attention(mars_kv_ctx* c, const mars_kv_cache* cache, 
     a.D = cache->head_dim; a.page = cache->page_size; a.num_pages = cache->num_pages; a.pitch = table_pitch;
     // The short kernel's tiles have 16 rows: with more it would read the keys once for
     // every 16, the chunk kernel once for every 256 but with three launches and tiles
-    // of 128 rows (64 ragged requests, 4 query heads a key head: 4 new tokens 202 us
-    // here, 5 there 259; 4 requests of 700 keys on the device: 11 us and 18).
+    // of 128 rows (64 ragged requests, 4 query heads a key head: 4 new tokens 208 us
+    // here, 5 there 273; 4 requests of 700 keys on the device: 11 us and 18).
     const bool chunk = (int64_t)std::max(cfg->max_new, 1) * a.group > kShortRows;
     MARS_TRY(kv_attn_memory(c, chunk));
     AttnWork w{};

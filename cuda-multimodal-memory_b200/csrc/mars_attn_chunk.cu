@@ -31,14 +31,20 @@
 // (prompts have thousands of units), a kernel after it joins cut units; their
 // set-ups overlap (programmatic dependent launch).
 //
-// Bound: 64 keys of the two row tiles take 1,280 cycles of products at D = 128
-// (S 16 x 48, read from shared memory at its full rate; O 8 x 64) and 1,024 of
-// exponentials (16 ex2 a cycle), measured alone; together a step takes 1,900
-// to 2,100, what is left being the way from weights to the next scores there
-// and back (arrive, product, commit, wait: 1,700 cycles) and both warpgroups
-// at their exponentials at once.  Measured: two prompts of 8,192 and 4,142
-// tokens, 32 heads on 8 of 128 columns, 843 us = 838 TFLOP/s at 1.55 GHz under
-// the power cap (the library's sustained rate for a plain product: 1,398).
+// Bound: the softmax warps.  64 keys of the two row tiles take 1,280 cycles of
+// products at D = 128 (S 16 x 48, read from shared memory at its full rate; O 8 x
+// 64) and 1,024 of exponentials (16 ex2 a cycle), measured alone; together a step
+// takes 1,900 to 2,200.  A trace of a prompt gives a warpgroup 1,190 of them for
+// exponentials, 290 for loading the scores and their maximum, 115 for rescaling
+// and 230 for waiting: two softmax warps a scheduler go through these one after
+// another, and tensor pipe and special function unit are each half busy.  Capped
+// scores with a decay took 4,450 cycles a step in the same trace, 2,200 of them
+// for the scores' shaping and maximum.  All variants are at their 168 registers
+// and spill 200 to 240 bytes.
+// Measured (bf16, 128 columns): two prompts of 8,192 and 4,142 tokens, 32 heads on
+// 8, 815 us = 867 TFLOP/s under the power cap (the library's sustained rate for a
+// plain product: 1,398).  8 chunks of up to 512 on up to 4,000, 16 heads on 4:
+// 98 us, with decay 140, with decay and cap 175, scores beyond half the cap 216.
 // Tried and dropped: exponentials on the FMA units beside the special function
 // unit (slower: 8 FMA cycles an element against 8 of ex2), the warpgroups held
 // out of step, one buffer of 128 keys' scores (915 us).
@@ -232,12 +238,11 @@ struct Walk {
 
 // A ring's next slot and the parity of its use.
 template <int kSlots> struct Ring {
-    int slot = 0, phase = 0, rounds = 0;
+    int slot = 0, phase = 0;
     __device__ __forceinline__ void step() {
         if (++slot == kSlots) {
             slot = 0;
             phase ^= 1;
-            ++rounds;
         }
     }
 };

@@ -26,8 +26,9 @@
 //    that a 128-key tile takes from HBM.
 //
 // Measured (bf16, D = 128): 64 requests of up to 8,000 keys, 32 heads on 8:
-// 207 us, 6.09 TB/s, 0.95 of the copy rate.  2 requests of up to 250,000, 16
-// heads on 4: 137 us, 0.87; there a unit is cut into 74 parts, and its joining
+// 201 us (198 to 212 from card to card), 6.28 TB/s, 0.97 of the copy rate; with a
+// cap of 30 203 us, scores beyond half of it 206.  2 requests of up to 250,000,
+// 16 heads on 4: 134 us, 0.89; there a unit is cut into 74 parts, and its joining
 // is what the other has not (it was 156 us with one thread a row to join).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

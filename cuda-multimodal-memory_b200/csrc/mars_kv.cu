@@ -11,8 +11,8 @@
 //
 // Both kernels do next to no arithmetic and move 4 to 12 bytes for each token
 // and page; what bounds them is the launch and the chain lengths -> prefix sum
-// -> page id -> slot (3 to 8 us on the device; a call from Python takes 19 us,
-// its host time).  So every block forms the prefix sums of all requests by
+// -> page id -> slot (4.6 us on the device for 64 requests with a token each, 10
+// for 300 prompts of 360,000 tokens; a call from Python takes 19 us, its host time).  So every block forms the prefix sums of all requests by
 // itself (at most 8,192 of them, 64 KB from L2) instead of waiting for another
 // launch, and finds a token's request by bisection in shared memory.  Inputs
 // and outputs may be the same arrays: the last block to arrive (a counter, no

@@ -17,10 +17,12 @@
 // Bound: HBM (every value is read and written once).  A block takes 1 to 4
 // tokens; threadIdx.x walks the 16-byte chunks of a head, threadIdx.y the
 // heads of q, k and v of all the block's tokens, so a warp covers whole
-// 128-byte lines on both sides; each thread has two 16-byte loads in flight
-// and full occupancy covers the latency.  Measured: 8,192 tokens of 32 + 8 + 8
-// heads of 128 in bf16 41 us, 4.9 TB/s, 0.76 of the copy rate; 16,381 tokens
-// of 12 heads of 64 in fp32 20.6 us, 0.76.  Loads issued one item ahead of the
+// 128-byte lines on both sides; each thread has two 16-byte loads in flight,
+// and 1,536 threads an SM (of 2,048: 33 to 40 registers) cover the latency.
+// Measured: 8,192 tokens of 32 + 8 + 8 heads of 128 in bf16 41 us, 4.9 TB/s, 0.76
+// of the copy rate; 16,381 tokens of 12 heads of 64 in fp32 20.6 us, 0.76.  Halves
+// that no 16-byte vector divides (72 or 120 columns in 16 bits) go by single
+// elements: the same 8,192 tokens with heads of 120 95 us, 0.31, of 72 83 us, 0.21.  Loads issued one item ahead of the
 // stores, the first beside the angles, were slower (53 us: more registers,
 // fewer blocks).
 #include <cuda_bf16.h>
